@@ -134,7 +134,8 @@ zrl_status zrl_create(const zrl_model_config *cfg, int device,
 /* Frees the context (the reference's ActorCritic is freed by Drop). */
 zrl_status zrl_destroy(zrl_ctx *ctx);
 /* The message of the last failure on ctx (where the reference panics, this
- * library returns a status and keeps the message here). */
+ * library returns a status and keeps the message here).  With ctx NULL: the
+ * message of the calling thread's last failed sequence-operator call. */
 const char *zrl_last_error(const zrl_ctx *ctx);
 /* ZRL_ABI_VERSION of the loaded library.  No counterpart in the reference. */
 int32_t zrl_abi_version(void);
@@ -363,6 +364,46 @@ int64_t zrl_rank_orders(uint64_t seed, int64_t n_global, int64_t n_local,
 zrl_status zrl_set_mirror(zrl_ctx *ctx, const int32_t *obs_perm, const float *obs_sign,
                           const int32_t *cobs_perm, const float *cobs_sign,
                           const int32_t *act_perm, const float *act_sign);
+
+/* ---- sequence operators ------------------------------------------------- */
+
+/* The parts of a policy with memory: what a recurrent actor-critic needs
+ * beside the MLP path above.  None has a counterpart in the reference, whose
+ * networks have no memory; episode ends cut their time axis as they cut
+ * gae's (ppo.rs:694-701).  Conventions:
+ *
+ *  - No context: every pointer to data is a device pointer on the current
+ *    device, and the work is queued on `stream` (a cudaStream_t; NULL for
+ *    the legacy default stream) without a host synchronization, so the calls
+ *    can be captured in a CUDA graph.  zrl_last_error(NULL) has the message
+ *    of this thread's last refusal.
+ *  - dtype (zrl_dtype) is the element type of the tensors declared void *;
+ *    sums, states, statistics and parameters are fp32.  Pointers are aligned
+ *    to their element, nothing more is asked; aligned rows run faster.
+ *  - strides, counted in elements, is a host array or NULL (every tensor
+ *    dense in the order its shape is written).  The last axis of every
+ *    tensor is dense.  Outputs do not overlap inputs or one another unless a
+ *    declaration says so, and an output's own elements do not overlap.
+ *  - Results do not depend on timing: no atomics on floating-point values.
+ */
+typedef enum { ZRL_F32 = 0, ZRL_BF16 = 1, ZRL_F16 = 2 } zrl_dtype;
+
+/* Dropout of x [N, D]: y = residual + x * keep / P(keep).  The mask is drawn
+ * from its coordinates and never stored: Philox4x32-10 under key (seed lo,
+ * seed hi) and counter (column / 8, row lo, row hi, stream_id) gives eight
+ * 16-bit lanes (the low half of each word first), one per column of the
+ * group; a value is kept where its lane is at least drop = round(65536 p)
+ * (ties to even), so P(keep) = 1 - drop / 65536 exactly.  rows [N] (or NULL
+ * for 0 .. N-1) numbers the rows, so a shuffled sample meets the mask that
+ * its rollout step drew.  The gradient of x is the same call on dy without a
+ * residual; the residual's gradient is dy.  A dropped value is not used: an
+ * infinity or NaN there gives 0 (+ residual).  strides: {x, residual, y}
+ * row strides.  y may be x or residual (same strides).  No counterpart in the
+ * reference. */
+zrl_status zrl_dropout(const void *x, const void *residual, const int64_t *rows,
+                       int64_t N, int64_t D, int32_t dtype, double p,
+                       uint64_t seed, uint32_t stream_id, const int64_t *strides,
+                       void *y, void *stream);
 
 /* ---- failure handling ---------------------------------------------------- */
 

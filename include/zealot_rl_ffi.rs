@@ -127,4 +127,8 @@ extern "C" {
                            gemm_launches: *mut i64) -> c_int;
     pub fn zrl_profile_site(ctx: *const ZrlCtx, i: i32, name: *mut *const c_char,
                             ms: *mut f32, spans: *mut i64) -> i32;
+    // sequence operators (device pointers, caller's stream, no context)
+    pub fn zrl_dropout(x: *const c_void, residual: *const c_void, rows: *const i64, n: i64,
+                       d: i64, dtype: i32, p: f64, seed: u64, stream_id: u32,
+                       strides: *const i64, y: *mut c_void, stream: *mut c_void) -> c_int;
 }

@@ -8,6 +8,7 @@
 #include <cuda_bf16.h>
 #include <stdint.h>
 
+#include "philox.cuh"
 #include "zrl_internal.h"
 
 namespace zrl {
@@ -1306,21 +1307,6 @@ __global__ void record_obs_kernel(const float *x, int64_t n, int dim,
 }
 
 // ------------------------------------------------------ rollout sampling
-
-// Philox4x32-10 (Salmon, Moraes, Dror, Shaw, "Parallel random numbers: as
-// easy as 1, 2, 3", SC'11): 10 rounds of the 4x32 S-box with the published
-// multipliers and Weyl key increments.
-__device__ __forceinline__ uint4 philox4x32_10(uint4 c, uint2 k) {
-#pragma unroll
-  for (int r = 0; r < 10; ++r) {
-    const uint32_t lo0 = 0xD2511F53u * c.x, hi0 = __umulhi(0xD2511F53u, c.x);
-    const uint32_t lo1 = 0xCD9E8D57u * c.z, hi1 = __umulhi(0xCD9E8D57u, c.z);
-    c = make_uint4(hi1 ^ c.y ^ k.x, lo1, hi0 ^ c.w ^ k.y, lo0);
-    k.x += 0x9E3779B9u;
-    k.y += 0xBB67AE85u;
-  }
-  return c;
-}
 
 // uniform in (0, 1): the top 24 bits, offset by half a step
 __device__ __forceinline__ float u01(uint32_t x) {

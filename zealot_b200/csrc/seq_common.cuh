@@ -1,0 +1,113 @@
+// seq_common.cuh -- what the sequence operators (dropout.cu, group_norm.cu,
+// gated_scan.cu) share: element types, vector loads and stores that convert
+// to and from fp32, and the refusal of bad arguments.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "zrl_internal.h"
+
+namespace zrl {
+
+// Records the calling thread's message (zrl_last_error(NULL)) and returns s.
+zrl_status seq_fail(zrl_status s, const char *fmt, ...)
+    __attribute__((format(printf, 2, 3)));
+// ZRL_OK, or the launch error of the calling thread's last kernel launch.
+zrl_status seq_launched(const char *what);
+
+inline int dtype_size(int32_t dt) { return dt == ZRL_F32 ? 4 : 2; }
+inline bool dtype_ok(int32_t dt) { return dt == ZRL_F32 || dt == ZRL_BF16 || dt == ZRL_F16; }
+inline bool aligned(const void *p, int64_t bytes) {
+  return (reinterpret_cast<uintptr_t>(p) % (uintptr_t)bytes) == 0;
+}
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+// Outputs are rounded once, to nearest even.
+template <typename T> __device__ __forceinline__ T from_f32(float v);
+template <> __device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) {
+  return __float2bfloat16_rn(v);
+}
+template <> __device__ __forceinline__ __half from_f32<__half>(float v) {
+  return __float2half_rn(v);
+}
+
+// V consecutive elements as one access (V * sizeof(T) in 2, 4, 8, 16 bytes,
+// aligned to that).
+template <int BYTES> struct RawT;
+template <> struct RawT<2> { using type = uint16_t; };
+template <> struct RawT<4> { using type = uint32_t; };
+template <> struct RawT<8> { using type = uint2; };
+template <> struct RawT<16> { using type = uint4; };
+template <typename T, int V> using Raw = typename RawT<V * (int)sizeof(T)>::type;
+
+template <typename T, int V>
+__device__ __forceinline__ void unpack(const Raw<T, V> &raw, float *out) {
+  if constexpr (sizeof(T) == 2 && V >= 2) {
+    const uint32_t *w = reinterpret_cast<const uint32_t *>(&raw);
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) {
+      if constexpr (sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value) {
+        out[2 * i] = __uint_as_float(w[i] << 16);
+        out[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+      } else {
+        const __half2 h = *reinterpret_cast<const __half2 *>(&w[i]);
+        const float2 f = __half22float2(h);
+        out[2 * i] = f.x;
+        out[2 * i + 1] = f.y;
+      }
+    }
+  } else {
+    const T *e = reinterpret_cast<const T *>(&raw);
+#pragma unroll
+    for (int i = 0; i < V; ++i) out[i] = to_f32(e[i]);
+  }
+}
+
+template <typename T, int V>
+__device__ __forceinline__ Raw<T, V> pack(const float *in) {
+  Raw<T, V> raw;
+  if constexpr (sizeof(T) == 2 && V >= 2) {
+    uint32_t *w = reinterpret_cast<uint32_t *>(&raw);
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) {
+      if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        const __nv_bfloat162 b = __floats2bfloat162_rn(in[2 * i], in[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t *>(&b);
+      } else {
+        const __half2 h = __floats2half2_rn(in[2 * i], in[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t *>(&h);
+      }
+    }
+  } else {
+    T *e = reinterpret_cast<T *>(&raw);
+#pragma unroll
+    for (int i = 0; i < V; ++i) e[i] = from_f32<T>(in[i]);
+  }
+  return raw;
+}
+
+template <typename T, int V>
+__device__ __forceinline__ void load_vec(const T *p, float *out) {
+  const Raw<T, V> raw = *reinterpret_cast<const Raw<T, V> *>(p);
+  unpack<T, V>(raw, out);
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_vec(T *p, const float *in) {
+  *reinterpret_cast<Raw<T, V> *>(p) = pack<T, V>(in);
+}
+
+// Calls f with a value of the element type that dtype names.
+template <typename F>
+inline void with_dtype(int32_t dtype, F &&f) {
+  if (dtype == ZRL_F32) f(float{});
+  else if (dtype == ZRL_BF16) f(__nv_bfloat16{});
+  else f(__half{});
+}
+
+}  // namespace zrl

@@ -1446,7 +1446,9 @@ zrl_status zrl_nccl_unique_id(uint8_t *out) {
 }
 
 const char *zrl_last_error(const zrl_ctx *ctx) {
-  return ctx ? ctx->err.c_str() : "null context";
+  if (ctx) return ctx->err.c_str();
+  const char *seq = seq_last_error();
+  return *seq ? seq : "null context";
 }
 
 zrl_status zrl_create(const zrl_model_config *cfg, int device,

@@ -22,6 +22,10 @@
 
 namespace zrl {
 
+// Message of this thread's last failed sequence-operator call (they take no
+// context); empty if there is none.
+const char *seq_last_error();
+
 constexpr int kPad = 32;
 inline int64_t pad_to(int64_t x, int64_t a) { return (x + a - 1) / a * a; }
 
