@@ -388,6 +388,81 @@ zrl_status zrl_set_mirror(zrl_ctx *ctx, const int32_t *obs_perm, const float *ob
  */
 typedef enum { ZRL_F32 = 0, ZRL_BF16 = 1, ZRL_F16 = 2 } zrl_dtype;
 
+/* A gated linear recurrence over T steps of B rows of D channels.  Per
+ * channel, with rate = c softplus(lam):
+ *     a_t = exp(-rate sigmoid(rec_t)), 0 where resets_t is not 0
+ *     h_t = a_t h_{t-1} + sqrt(1 - a_t^2) sigmoid(inp_t) x_t
+ * h_{-1} = h0 [B, D] (NULL: zeros).  resets [B, T] (bytes, or NULL) marks
+ * the steps at which an episode begins; the state before it is not used, not
+ * even an infinity or NaN.  x, rec, inp, h: [B, T, D].  h_last [B, D] (or
+ * NULL) gets the last state, h0 where T is 0; it may be h0 itself, which is
+ * the rollout's single step: T = 1, the state updated in place.  carry (or
+ * NULL where no gradient follows) gets zrl_gated_scan_carry() floats: the
+ * states at steps 64, 128, ...  strides: (batch, time) of x, rec, inp,
+ * resets and h, ten in all.  No counterpart in the reference. */
+zrl_status zrl_gated_scan(const void *x, const void *rec, const void *inp,
+                          const float *lam, const float *h0, const uint8_t *resets,
+                          int64_t B, int64_t T, int64_t D, int32_t dtype, float c,
+                          const int64_t *strides, void *h, float *h_last,
+                          float *carry, void *stream);
+/* Floats in zrl_gated_scan's carry: B * D for every 64 steps after the
+ * first 64.  No counterpart in the reference. */
+int64_t zrl_gated_scan_carry(int64_t B, int64_t T, int64_t D);
+/* The gradient of zrl_gated_scan, for dh [B, T, D] on h and dh_last [B, D]
+ * (or NULL) on h_last: dx, drec, dinp [B, T, D], dlam [D], dh0 [B, D] (or
+ * NULL).  The other arguments are the forward call's, carry what it wrote
+ * (NULL is accepted up to 64 steps).  Where 1 - a^2 is 0 in 32 bits the term
+ * of the square root's slope is left out of drec and dlam.  strides: (batch,
+ * time) of x, rec, inp, resets, dh, dx, drec and dinp, sixteen in all.
+ * workspace: zrl_gated_scan_grad_workspace() bytes, 16-byte aligned.  No
+ * counterpart in the reference. */
+zrl_status zrl_gated_scan_grad(const void *x, const void *rec, const void *inp,
+                               const float *lam, const float *h0,
+                               const uint8_t *resets, const float *carry,
+                               const void *dh, const float *dh_last, int64_t B,
+                               int64_t T, int64_t D, int32_t dtype, float c,
+                               const int64_t *strides, void *dx, void *drec,
+                               void *dinp, float *dlam, float *dh0,
+                               void *workspace, int64_t workspace_bytes,
+                               void *stream);
+/* Bytes of zrl_gated_scan_grad's workspace.  No counterpart in the
+ * reference. */
+int64_t zrl_gated_scan_grad_workspace(int64_t B, int64_t T, int64_t D);
+
+/* Activations of zrl_group_norm: z, ELU (alpha 1), z sigmoid(z), z Phi(z). */
+typedef enum {
+  ZRL_ACT_NONE = 0, ZRL_ACT_ELU = 1, ZRL_ACT_SILU = 2, ZRL_ACT_GELU = 3
+} zrl_activation;
+
+/* Group norm with an activation over channels-last x [N, L, C]: per n and
+ * group of C / groups neighbouring channels, over the L rows (positions; 1
+ * normalizes every row by itself), y = act(gamma (x - mean) rstd + beta),
+ * rstd = 1 / sqrt(population variance + eps).  gamma, beta [C] fp32 or NULL
+ * (1, 0).  mean, rstd [N, groups] or NULL: what the gradient needs.  strides:
+ * (n, l) of x and y, four in all.  y may be x (same strides).  workspace:
+ * zrl_group_norm_workspace(..., 0) bytes, 16-byte aligned (NULL if 0).  No
+ * counterpart in the reference. */
+zrl_status zrl_group_norm(const void *x, const float *gamma, const float *beta,
+                          int64_t N, int64_t L, int64_t C, int32_t groups,
+                          int32_t dtype, int32_t act, float eps,
+                          const int64_t *strides, void *y, float *mean, float *rstd,
+                          void *workspace, int64_t workspace_bytes, void *stream);
+/* The gradient of zrl_group_norm for dy [N, L, C]: dx, and dgamma, dbeta [C]
+ * (or NULL).  strides: (n, l) of x, dy and dx, six in all.  dx may be dy
+ * (same strides).  workspace: zrl_group_norm_workspace(..., 1) bytes, 16-byte
+ * aligned.  No counterpart in the reference. */
+zrl_status zrl_group_norm_grad(const void *x, const void *dy, const float *gamma,
+                               const float *beta, const float *mean,
+                               const float *rstd, int64_t N, int64_t L, int64_t C,
+                               int32_t groups, int32_t dtype, int32_t act,
+                               const int64_t *strides, void *dx, float *dgamma,
+                               float *dbeta, void *workspace,
+                               int64_t workspace_bytes, void *stream);
+/* Bytes of the workspace of zrl_group_norm (grad 0) or zrl_group_norm_grad
+ * (grad 1).  No counterpart in the reference. */
+int64_t zrl_group_norm_workspace(int64_t N, int64_t L, int64_t C, int32_t groups,
+                                 int32_t grad);
+
 /* Dropout of x [N, D]: y = residual + x * keep / P(keep).  The mask is drawn
  * from its coordinates and never stored: Philox4x32-10 under key (seed lo,
  * seed hi) and counter (column / 8, row lo, row hi, stream_id) gives eight

@@ -128,6 +128,31 @@ extern "C" {
     pub fn zrl_profile_site(ctx: *const ZrlCtx, i: i32, name: *mut *const c_char,
                             ms: *mut f32, spans: *mut i64) -> i32;
     // sequence operators (device pointers, caller's stream, no context)
+    pub fn zrl_gated_scan(x: *const c_void, rec: *const c_void, inp: *const c_void,
+                          lam: *const f32, h0: *const f32, resets: *const u8, b: i64, t: i64,
+                          d: i64, dtype: i32, c: f32, strides: *const i64, h: *mut c_void,
+                          h_last: *mut f32, carry: *mut f32, stream: *mut c_void) -> c_int;
+    pub fn zrl_gated_scan_carry(b: i64, t: i64, d: i64) -> i64;
+    pub fn zrl_gated_scan_grad(x: *const c_void, rec: *const c_void, inp: *const c_void,
+                               lam: *const f32, h0: *const f32, resets: *const u8,
+                               carry: *const f32, dh: *const c_void, dh_last: *const f32,
+                               b: i64, t: i64, d: i64, dtype: i32, c: f32, strides: *const i64,
+                               dx: *mut c_void, drec: *mut c_void, dinp: *mut c_void,
+                               dlam: *mut f32, dh0: *mut f32, workspace: *mut c_void,
+                               workspace_bytes: i64, stream: *mut c_void) -> c_int;
+    pub fn zrl_gated_scan_grad_workspace(b: i64, t: i64, d: i64) -> i64;
+    pub fn zrl_group_norm(x: *const c_void, gamma: *const f32, beta: *const f32, n: i64, l: i64,
+                          c: i64, groups: i32, dtype: i32, act: i32, eps: f32,
+                          strides: *const i64, y: *mut c_void, mean: *mut f32, rstd: *mut f32,
+                          workspace: *mut c_void, workspace_bytes: i64,
+                          stream: *mut c_void) -> c_int;
+    pub fn zrl_group_norm_grad(x: *const c_void, dy: *const c_void, gamma: *const f32,
+                               beta: *const f32, mean: *const f32, rstd: *const f32, n: i64,
+                               l: i64, c: i64, groups: i32, dtype: i32, act: i32,
+                               strides: *const i64, dx: *mut c_void, dgamma: *mut f32,
+                               dbeta: *mut f32, workspace: *mut c_void, workspace_bytes: i64,
+                               stream: *mut c_void) -> c_int;
+    pub fn zrl_group_norm_workspace(n: i64, l: i64, c: i64, groups: i32, grad: i32) -> i64;
     pub fn zrl_dropout(x: *const c_void, residual: *const c_void, rows: *const i64, n: i64,
                        d: i64, dtype: i32, p: f64, seed: u64, stream_id: u32,
                        strides: *const i64, y: *mut c_void, stream: *mut c_void) -> c_int;

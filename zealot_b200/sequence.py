@@ -20,6 +20,9 @@ import torch
 
 from . import native as N
 
+#: what ``act`` of group_norm may be
+ACTIVATIONS = {"none": 0, "elu": 1, "silu": 2, "gelu": 3}
+
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
@@ -63,6 +66,245 @@ def _row_stride(name, t, D):
     except RuntimeError:
         raise _invalid(f"{name}: the leading axes do not merge into one row axis") from None
     return v.stride(0)
+
+
+def _f32(name, t, shape, device):
+    """The address of an fp32 parameter, state or statistic; None stays None."""
+    if t is None:
+        return None
+    _same(name, t, shape, torch.float32, device)
+    if not t.is_contiguous():
+        raise _invalid(f"{name}: not contiguous")
+    return t.data_ptr()
+
+
+def _bt(name, t):
+    """(batch, time) strides of a [B, T, D] tensor whose last axis is dense."""
+    if t.shape[2] > 1 and t.stride(2) != 1:
+        raise _invalid(f"{name}: the last axis is not dense")
+    return t.stride(0), t.stride(1)
+
+
+def _like(x):
+    """An empty tensor of x's shape: time-major in memory where x is."""
+    B, T, D = x.shape
+    if x.stride(0) < x.stride(1) and B > 1 and T > 1:
+        return torch.empty((T, B, D), dtype=x.dtype, device=x.device).transpose(0, 1)
+    return torch.empty((B, T, D), dtype=x.dtype, device=x.device)
+
+
+def _scan_inputs(x, rec, inp, lam, h0, resets, shape):
+    """Checks what forward and gradient share; (lam, h0, resets) addresses."""
+    dev = x.device
+    _same("rec", rec, shape, x.dtype, dev)
+    _same("inp", inp, shape, x.dtype, dev)
+    D = shape[-1]
+    if resets is not None:
+        if resets.dtype not in (torch.uint8, torch.bool) or resets.device != dev:
+            raise TypeError("resets: uint8 or bool on x's device")
+        if resets.shape != shape[:-1]:
+            raise _invalid(f"resets: shape {tuple(resets.shape)}, expected {tuple(shape[:-1])}")
+    return (_f32("lam", lam, (D,), dev), _f32("h0", h0, (shape[0], D), dev),
+            None if resets is None else resets.data_ptr())
+
+
+def _strides(tensors, resets):
+    """The (batch, time) strides of the call's tensors with resets' in fourth
+    place, or None where all are dense in [B, T, D] order."""
+    if all(t.is_contiguous() for _, t in tensors) and (resets is None or resets.is_contiguous()):
+        return None
+    st = []
+    for i, (name, t) in enumerate(tensors):
+        if i == 3:
+            st += (0, 0) if resets is None else resets.stride()
+        st += _bt(name, t)
+    return (C.c_int64 * len(st))(*st)
+
+
+def gated_scan(x, rec, inp, lam, h0=None, resets=None, c: float = 8.0, save: bool = False,
+               out=None):
+    """A gated linear recurrence over the time axis of [B, T, D] tensors.
+
+    With rate = c softplus(lam):
+        a_t = exp(-rate sigmoid(rec_t)), 0 where resets_t is set
+        h_t = a_t h_{t-1} + sqrt(1 - a_t^2) sigmoid(inp_t) x_t
+    from h_{-1} = h0 (float32 [B, D]; zeros by default).  ``resets`` (uint8 or
+    bool [B, T]) marks the steps at which an episode begins; a step's mark is
+    the ``done`` of the step before it.  Several recordings laid end to end in
+    one row are marked the same way.  x, rec and inp may be slices of one
+    projection's output and in any order of batch and time.
+
+    Returns (h, h_last): h in x's type, h_last float32 [B, D].  With ``save``
+    also the carry that ``gated_scan_grad`` takes."""
+    if x.dim() != 3:
+        raise _invalid(f"x: {x.dim()} axes, expected [B, T, D]")
+    dt, dev, shape = _dtype(x), x.device, x.shape
+    p_lam, p_h0, p_z = _scan_inputs(x, rec, inp, lam, h0, resets, shape)
+    B, T, D = shape
+    if out is None:
+        out = _like(x)
+    else:
+        _same("out", out, shape, x.dtype, dev)
+    last = torch.empty((B, D), dtype=torch.float32, device=dev)
+    carry = None
+    if save:
+        carry = torch.empty((B, max(T - 1, 0) // 64, D), dtype=torch.float32, device=dev)
+    st = _strides((("x", x), ("rec", rec), ("inp", inp), ("out", out)), resets)
+    _call(N.lib().zrl_gated_scan, dev, x.data_ptr(), rec.data_ptr(), inp.data_ptr(), p_lam,
+          p_h0, p_z, B, T, D, dt, c, st, out.data_ptr(), last.data_ptr(),
+          carry.data_ptr() if save else None)
+    return (out, last, carry) if save else (out, last)
+
+
+def gated_step(x, rec, inp, lam, state, resets=None, c: float = 8.0, out=None):
+    """One step of ``gated_scan`` for a rollout: x, rec, inp [B, D], state
+    float32 [B, D], resets [B].  Returns (h, new state); ``out=state`` updates
+    the state in place."""
+    if x.dim() != 2:
+        raise _invalid(f"x: {x.dim()} axes, expected [B, D]")
+    dt, dev, shape = _dtype(x), x.device, x.shape
+    if state is None:
+        raise _invalid("state: a float32 tensor [B, D]")
+    p_lam, p_h0, p_z = _scan_inputs(x, rec, inp, lam, state, resets, shape)
+    B, D = shape
+    h = torch.empty((B, D), dtype=x.dtype, device=dev)
+    if out is None:
+        out = torch.empty((B, D), dtype=torch.float32, device=dev)
+    st = None
+    if not (x.is_contiguous() and rec.is_contiguous() and inp.is_contiguous() and
+            (resets is None or resets.is_contiguous())):
+        if D > 1 and any(t.stride(1) != 1 for t in (x, rec, inp)):
+            raise _invalid("x, rec, inp: the last axis is not dense")
+        z = resets.stride(0) if resets is not None else 0
+        st = (C.c_int64 * 10)(x.stride(0), 0, rec.stride(0), 0, inp.stride(0), 0, z, 0, D, 0)
+    _call(N.lib().zrl_gated_scan, dev, x.data_ptr(), rec.data_ptr(), inp.data_ptr(), p_lam,
+          p_h0, p_z, B, 1, D, dt, c, st, h.data_ptr(), _f32("out", out, (B, D), dev), None)
+    return h, out
+
+
+def gated_scan_grad(x, rec, inp, lam, dh, carry, dh_last=None, h0=None, resets=None,
+                    c: float = 8.0, out=None):
+    """The gradient of ``gated_scan`` for dh on h and dh_last on h_last.
+
+    ``carry`` is what the forward call with ``save`` returned; the other
+    arguments are that call's.  Returns (dx, drec, dinp, dlam, dh0), dh0 None
+    without h0.  ``out``: three tensors for dx, drec and dinp, such as slices
+    of one buffer for the projection's gradient."""
+    if x.dim() != 3:
+        raise _invalid(f"x: {x.dim()} axes, expected [B, T, D]")
+    dt, dev, shape = _dtype(x), x.device, x.shape
+    p_lam, p_h0, p_z = _scan_inputs(x, rec, inp, lam, h0, resets, shape)
+    B, T, D = shape
+    _same("dh", dh, shape, x.dtype, dev)
+    p_dl = _f32("dh_last", dh_last, (B, D), dev)
+    p_c = _f32("carry", carry, (B, max(T - 1, 0) // 64, D), dev)
+    if out is None:
+        out = _like(x), _like(x), _like(x)
+    else:
+        for name, t in zip(("dx", "drec", "dinp"), out, strict=True):
+            _same(name, t, shape, x.dtype, dev)
+    dx, drec, dinp = out
+    dlam = torch.empty(D, dtype=torch.float32, device=dev)
+    dh0 = None if h0 is None else torch.empty((B, D), dtype=torch.float32, device=dev)
+    lib = N.lib()
+    nw = lib.zrl_gated_scan_grad_workspace(B, T, D)
+    ws = torch.empty(nw, dtype=torch.uint8, device=dev)
+    st = _strides((("x", x), ("rec", rec), ("inp", inp), ("dh", dh), ("dx", dx), ("drec", drec),
+                   ("dinp", dinp)), resets)
+    _call(lib.zrl_gated_scan_grad, dev, x.data_ptr(), rec.data_ptr(), inp.data_ptr(), p_lam,
+          p_h0, p_z, p_c, dh.data_ptr(), p_dl, B, T, D, dt, c, st, dx.data_ptr(),
+          drec.data_ptr(), dinp.data_ptr(), dlam.data_ptr(),
+          None if dh0 is None else dh0.data_ptr(), ws.data_ptr(), nw)
+    return dx, drec, dinp, dlam, dh0
+
+
+def _nl(name, t):
+    """(n, l) strides of channels-last [N, ..., C], the middle axes as one."""
+    if t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise _invalid(f"{name}: the last axis is not dense")
+    if t.dim() == 2:
+        return t.stride(0), t.shape[1]
+    if t.dim() == 3:
+        return t.stride(0), t.stride(1)
+    try:
+        v = t.view(t.shape[0], -1, t.shape[-1])
+    except RuntimeError:
+        raise _invalid(f"{name}: the middle axes do not merge into one") from None
+    return v.stride(0), v.stride(1)
+
+
+def _norm_shape(x, groups, act):
+    """(dtype, N, L, C, act) of a group-norm call."""
+    if x.dim() < 2:
+        raise _invalid("x: [N, C] or [N, ..., C]")
+    dt, Cn = _dtype(x), x.shape[-1]
+    if groups < 1 or Cn % groups:
+        raise _invalid(f"{Cn} channels in {groups} groups")
+    if act not in ACTIVATIONS:
+        raise _invalid(f"activation {act!r}: one of {', '.join(ACTIVATIONS)}")
+    L = 1
+    for n in x.shape[1:-1]:
+        L *= n
+    return dt, x.shape[0], L, Cn, ACTIVATIONS[act]
+
+
+def _norm_strides(tensors):
+    if all(t.is_contiguous() for _, t in tensors) or not tensors[0][1].numel():
+        return None
+    st = [v for name, t in tensors for v in _nl(name, t)]
+    return (C.c_int64 * len(st))(*st)
+
+
+def group_norm(x, groups: int, gamma=None, beta=None, act: str = "elu", eps: float = 1e-5,
+               save: bool = False, out=None):
+    """Group norm over channels-last x [N, ..., C] and an activation.
+
+    Each n and each of ``groups`` groups of neighbouring channels is
+    normalized over its channels and all middle axes; [N, C] normalizes each
+    row by itself, which is the form for time steps (nothing of a later step
+    reaches an earlier one).  gamma, beta: float32 [C] or None.  ``act`` is one
+    of ``ACTIVATIONS``.  ``out`` may be x.  Returns y, and with ``save`` also
+    (mean, rstd), float32 [N, groups]."""
+    dt, n, L, Cn, a = _norm_shape(x, groups, act)
+    dev = x.device
+    p_g, p_b = _f32("gamma", gamma, (Cn,), dev), _f32("beta", beta, (Cn,), dev)
+    if out is None:
+        out = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    else:
+        _same("out", out, x.shape, x.dtype, dev)
+    mean = rstd = None
+    if save:
+        mean, rstd = torch.empty((2, n, groups), dtype=torch.float32, device=dev).unbind(0)
+    lib = N.lib()
+    nw = lib.zrl_group_norm_workspace(n, L, Cn, groups, 0)
+    ws = torch.empty(nw, dtype=torch.uint8, device=dev) if nw else None
+    _call(lib.zrl_group_norm, dev, x.data_ptr(), p_g, p_b, n, L, Cn, groups, dt, a, eps,
+          _norm_strides((("x", x), ("out", out))), out.data_ptr(),
+          mean.data_ptr() if save else None, rstd.data_ptr() if save else None,
+          ws.data_ptr() if nw else None, nw)
+    return (out, mean, rstd) if save else out
+
+
+def group_norm_grad(x, dy, groups: int, gamma, beta, mean, rstd, act: str = "elu", out=None):
+    """The gradient of ``group_norm`` for dy: (dx, dgamma, dbeta).  mean and
+    rstd are the forward call's; ``out`` (for dx) may be dy."""
+    dt, n, L, Cn, a = _norm_shape(x, groups, act)
+    dev = x.device
+    _same("dy", dy, x.shape, x.dtype, dev)
+    p_g, p_b = _f32("gamma", gamma, (Cn,), dev), _f32("beta", beta, (Cn,), dev)
+    p_m, p_r = _f32("mean", mean, (n, groups), dev), _f32("rstd", rstd, (n, groups), dev)
+    if out is None:
+        out = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    else:
+        _same("out", out, x.shape, x.dtype, dev)
+    dgamma, dbeta = torch.empty((2, Cn), dtype=torch.float32, device=dev).unbind(0)
+    lib = N.lib()
+    nw = lib.zrl_group_norm_workspace(n, L, Cn, groups, 1)
+    ws = torch.empty(nw, dtype=torch.uint8, device=dev) if nw else None
+    _call(lib.zrl_group_norm_grad, dev, x.data_ptr(), dy.data_ptr(), p_g, p_b, p_m, p_r, n, L,
+          Cn, groups, dt, a, _norm_strides((("x", x), ("dy", dy), ("out", out))),
+          out.data_ptr(), dgamma.data_ptr(), dbeta.data_ptr(), ws.data_ptr() if nw else None, nw)
+    return out, dgamma, dbeta
 
 
 def dropout(x, p: float, seed: int, stream: int = 0, rows=None, residual=None, out=None):
