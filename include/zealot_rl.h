@@ -398,20 +398,20 @@ typedef enum { ZRL_F32 = 0, ZRL_BF16 = 1, ZRL_F16 = 2 } zrl_dtype;
  * NULL) gets the last state, h0 where T is 0; it may be h0 itself, which is
  * the rollout's single step: T = 1, the state updated in place.  carry (or
  * NULL where no gradient follows) gets zrl_gated_scan_carry() floats: the
- * states at steps 64, 128, ...  strides: (batch, time) of x, rec, inp,
+ * states before steps 8, 16, ...  strides: (batch, time) of x, rec, inp,
  * resets and h, ten in all.  No counterpart in the reference. */
 zrl_status zrl_gated_scan(const void *x, const void *rec, const void *inp,
                           const float *lam, const float *h0, const uint8_t *resets,
                           int64_t B, int64_t T, int64_t D, int32_t dtype, float c,
                           const int64_t *strides, void *h, float *h_last,
                           float *carry, void *stream);
-/* Floats in zrl_gated_scan's carry: B * D for every 64 steps after the
- * first 64.  No counterpart in the reference. */
+/* Floats in zrl_gated_scan's carry: B * D for every 8 steps after the
+ * first 8.  No counterpart in the reference. */
 int64_t zrl_gated_scan_carry(int64_t B, int64_t T, int64_t D);
 /* The gradient of zrl_gated_scan, for dh [B, T, D] on h and dh_last [B, D]
  * (or NULL) on h_last: dx, drec, dinp [B, T, D], dlam [D], dh0 [B, D] (or
  * NULL).  The other arguments are the forward call's, carry what it wrote
- * (NULL is accepted up to 64 steps).  Where 1 - a^2 is 0 in 32 bits the term
+ * (NULL is accepted up to 8 steps).  Where 1 - a^2 is 0 in 32 bits the term
  * of the square root's slope is left out of drec and dlam.  strides: (batch,
  * time) of x, rec, inp, resets, dh, dx, drec and dinp, sixteen in all.
  * workspace: zrl_gated_scan_grad_workspace() bytes, 16-byte aligned.  No

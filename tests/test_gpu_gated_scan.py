@@ -389,6 +389,6 @@ def test_refusals_without_a_gpu():
 
     for kw in (dict(t=65), dict(ws=None), dict(nbytes=0), dict(dlam=None), dict(dx=None)):
         assert grad(**kw) == N.INVALID_ARG, kw
-    assert L.zrl_gated_scan_carry(2, 64, 4) == 0
-    assert L.zrl_gated_scan_carry(2, 65, 4) == 8
-    assert L.zrl_gated_scan_carry(2, 129, 4) == 16
+    assert L.zrl_gated_scan_carry(2, 8, 4) == 0
+    assert L.zrl_gated_scan_carry(2, 9, 4) == 8
+    assert L.zrl_gated_scan_carry(2, 17, 4) == 16

@@ -11,20 +11,22 @@
 #include <math.h>
 
 #include <algorithm>
-#include <initializer_list>
 #include <type_traits>
 
 #include "seq_common.cuh"
 
+#ifndef ROWS_GROUPS
+#define ROWS_GROUPS 148 * 16
+#endif
 namespace zrl {
 namespace {
 
-constexpr int kSteps = 8;       // steps one warp takes from a tile
+constexpr int kSteps = 8;       // steps of a stretch
 constexpr int kWarps = 8;       // warps of a block at most
 constexpr int kMaxCluster = 16;
-// A tile of a long row: kWarps x kSteps steps.  The forward call keeps the
-// state at every kChunk-th step, where the gradient's tiles start from.
-constexpr int kChunk = kSteps * kWarps;
+// The forward call keeps the state before every stretch after the first; the
+// gradient recomputes the states inside a stretch from there.
+constexpr int kChunk = kSteps;
 constexpr float kLog2e = 1.44269504f;
 constexpr float kSeriesMax = 0.35f;
 constexpr float kTinySquare = 7.5231638e-37f;  // 2^-120
@@ -37,7 +39,8 @@ struct ScanArgs {
   float *h_last, *carry, *dh0, *part;
   int64_t B, T, D, K;   // K: chunk starts after the first
   int64_t units, tiles; // units of V channels; tiles of one row
-  int64_t xb, xt, rb, rt, ib, it, zb, zt, hb, ht, gb, gt, dxb, dxt, drb, drt, dib, dit;
+  int64_t xb, rb, ib, zb, zt, hb, gb, dxb, drb, dib;  // strides, elements
+  int32_t xt, rt, it, ht, gt, dxt, drt, dit;          // strides along time, bytes
   float c;
 };
 
@@ -74,21 +77,17 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 // One element's gates.  With u = rate sigmoid(rec), e = 1 - a = 1 - exp(-u)
 // comes from its series up to u = 0.35 (seven terms, 2e-8 relative): a = 1 - e
 // is then within half a unit of exp(-u) at every step, so the roundings of a
-// long memory do not add up in one direction, and 1 - a^2 = e (2 - e) keeps its
-// digits where a is near 1.  Above (only SLOW looks), a comes from ex2.
-// m sigmoid(inp) = s / sqrt(s q^2) with s = 1 - a^2, q = 1 + exp(-inp): one
-// reciprocal square root for the square root and the quotient.  exp(-inp) is
-// held to 2^60, exp(-rec) to 2^126 and s to at least 2^-120, so nothing
+// long memory do not add up in one direction, and s = 1 - a^2 = e (2 - e)
+// keeps its digits where a is near 1.  Above (only SLOW looks), a comes from
+// ex2.  exp(-rec) is held to 2^126 and s to at least 2^-120, so nothing
 // overflows or divides by zero.
-struct Gate {
-  float sr, e, s, q, ms;  // sigmoid(rec), 1 - a, 1 - a^2, 1 + exp(-inp), m sigmoid(inp)
-  float w;                // 1 / (sqrt(s) q)
+struct Decay {
+  float sr, e;  // sigmoid(rec), 1 - a
 };
 template <bool SLOW>
-__device__ __forceinline__ Gate gate(float rec, float inp, float rate, bool reset) {
-  Gate g;
+__device__ __forceinline__ Decay decay(float rec, float rate, bool reset) {
+  Decay g;
   g.sr = rcp(1.0f + ex2(min_nan(rec * -kLog2e, 126.0f)));
-  g.q = 1.0f + ex2(min_nan(inp * -kLog2e, 60.0f));
   const float u = rate * g.sr;
   float p = fmaf(u, 1.0f / 5040.0f, -1.0f / 720.0f);
   p = fmaf(u, p, 1.0f / 120.0f);
@@ -101,10 +100,21 @@ __device__ __forceinline__ Gate gate(float rec, float inp, float rate, bool rese
     if (u > kSeriesMax) g.e = 1.0f - ex2(u * -kLog2e);
     if (reset) g.e = 1.0f;  // a = 0, m = 1
   }
-  g.s = max_nan(fmaf(-g.e, g.e, 2.0f * g.e), kTinySquare);
-  g.w = rsq(g.s * g.q * g.q);
-  g.ms = g.s * g.w;
   return g;
+}
+// m sigmoid(inp) = s w with w = 1 / sqrt(s q^2), q = 1 + exp(-inp): one
+// reciprocal square root for the square root and the quotient.  exp(-inp) is
+// held to 2^60.
+struct Feed {
+  float ms, w, q;
+};
+__device__ __forceinline__ Feed feed(float inp, float e) {
+  Feed f;
+  f.q = 1.0f + ex2(min_nan(inp * -kLog2e, 60.0f));
+  const float s = max_nan(fmaf(-e, e, 2.0f * e), kTinySquare);
+  f.w = rsq(s * f.q * f.q);
+  f.ms = s * f.w;
+  return f;
 }
 
 // A stretch of steps maps the state before it to h -> P h + H.  P is -0 where
@@ -136,6 +146,22 @@ __device__ __forceinline__ void store_pair_at(float2 *p, uint32_t rank, float2 v
                : "memory");
 }
 
+// Element (row b, step t, channel d) of a [B, T, D] tensor; the steps of a stretch
+// follow by adding the stride.
+template <typename T>
+__device__ __forceinline__ const char *at_step(const void *p, int64_t b, int64_t sb, int64_t t,
+                                               int32_t st, int64_t d) {
+  return static_cast<const char *>(p) + (b * sb + d) * (int64_t)sizeof(T) + t * st;
+}
+template <typename T, int V>
+__device__ __forceinline__ Raw<T, V> load_step(const char *p) {
+  return *reinterpret_cast<const Raw<T, V> *>(p);
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_step(const char *p, const float *v) {
+  *reinterpret_cast<Raw<T, V> *>(const_cast<char *>(p)) = pack<T, V>(v);
+}
+
 // The reset marks of steps t .. t + n - 1 of the lane's row, bit s for step s.
 // A warp whose lanes share a row reads each mark once.
 __device__ __forceinline__ uint32_t reset_bits(const ScanArgs &a, int64_t b, int64_t t, int n,
@@ -148,6 +174,7 @@ __device__ __forceinline__ uint32_t reset_bits(const ScanArgs &a, int64_t b, int
     const bool on = lane < n && z[lane * a.zt];
     bits = __ballot_sync(0xffffffffu, on);
   } else {
+#pragma unroll 1
     for (int s = 0; s < n; ++s) bits |= (z[s * a.zt] ? 1u : 0u) << s;
   }
   return bits;
@@ -172,51 +199,134 @@ struct Place {
   }
 };
 
-// Blocks of 32 lanes x W warps along time x Z groups of lanes.  A tile is W
-// times S steps: every warp folds its S steps from a zero state in registers,
-// the warps (and, through distributed shared memory, the blocks of a cluster,
-// which take neighbouring tiles) exchange (P, H), and every warp runs its
-// steps again from its true state and stores them.  One pass over the data.
-template <typename T, int V, int S>
-__global__ void __launch_bounds__(256) scan_kernel(const __grid_constant__ ScanArgs a) {
-  __shared__ float2 agg[2][kWarps][32 * V];
-  __shared__ float2 cagg[2][kMaxCluster][32 * V];
-  const int lane = threadIdx.x, wt = threadIdx.y, W = blockDim.y;
-  const int slot = threadIdx.z * W;
-  const uint32_t ranks = cluster_size(), rank = cluster_rank();
-  const Place<V> at(a, ((int64_t)(blockIdx.x / ranks) * blockDim.z + threadIdx.z) * 32 + lane);
-  float rate[V], carry[V];
+template <int V>
+__device__ __forceinline__ bool load_rates(const ScanArgs &a, const Place<V> &at, float *rate) {
   bool big = false;
 #pragma unroll
   for (int v = 0; v < V; ++v) {
     rate[v] = a.c * softplus(a.lam[at.d + v]);
     big |= rate[v] > kSeriesMax;
-    carry[v] = a.h0 ? a.h0[at.b * a.D + at.d + v] : 0.0f;
   }
-  big = __any_sync(0xffffffffu, big);
-  const T *xp = static_cast<const T *>(a.x) + at.b * a.xb + at.d;
-  const T *rp = static_cast<const T *>(a.rec) + at.b * a.rb + at.d;
-  const T *ip = static_cast<const T *>(a.inp) + at.b * a.ib + at.d;
-  T *hp = static_cast<T *>(a.h) + at.b * a.hb + at.d;
+  return __any_sync(0xffffffffu, big);
+}
+
+// Rows in one piece: a thread takes its V channels through all steps, with the
+// loads of the S steps ahead in flight.
+template <typename T, int V, int S>
+__global__ void __launch_bounds__(256) scan_rows_kernel(const __grid_constant__ ScanArgs a) {
+  const Place<V> at(a, ((int64_t)blockIdx.x * blockDim.z + threadIdx.z) * 32 + threadIdx.x);
+  Raw<T, V> rr[S], ri[S], rx[S];
+  const char *rp = at_step<T>(a.rec, at.b, a.rb, 0, a.rt, at.d);
+  const char *ip = at_step<T>(a.inp, at.b, a.ib, 0, a.it, at.d);
+  const char *xp = at_step<T>(a.x, at.b, a.xb, 0, a.xt, at.d);
+#pragma unroll
+  for (int s = 0; s < S; ++s) {
+    rr[s] = ri[s] = rx[s] = Raw<T, V>{};
+    if (s < a.T) {
+      rr[s] = load_step<T, V>(rp);
+      ri[s] = load_step<T, V>(ip);
+      rx[s] = load_step<T, V>(xp);
+    }
+    rp += a.rt, ip += a.it, xp += a.xt;
+  }
+  float h[V], rate[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) h[v] = a.h0 ? a.h0[at.b * a.D + at.d + v] : 0.0f;
+  const bool big = load_rates<V>(a, at, rate);
+  const char *hp = at_step<T>(a.h, at.b, a.hb, 0, a.ht, at.d);
+  for (int64_t t0 = 0; t0 < a.T; t0 += S) {
+    const int n = (int)min((int64_t)S, a.T - t0);
+    const int ahead = (int)max((int64_t)0, min((int64_t)S, a.T - t0 - S));
+    const uint32_t z = reset_bits(a, at.b, t0, n, at.one_row);
+    if (a.carry && t0 && at.live) {
+#pragma unroll
+      for (int v = 0; v < V; ++v)
+        a.carry[(at.b * a.K + t0 / kChunk - 1) * a.D + at.d + v] = h[v];
+    }
+    auto run = [&](auto tag) {
+      constexpr bool SLOW = decltype(tag)::value;
+#pragma unroll
+      for (int s = 0; s < S; ++s) {
+        if (SLOW && s >= n) break;
+        float r[V], i[V], x[V];
+        unpack<T, V>(rr[s], r);
+        unpack<T, V>(ri[s], i);
+        unpack<T, V>(rx[s], x);
+        if (s < ahead) {
+          rr[s] = load_step<T, V>(rp);
+          ri[s] = load_step<T, V>(ip);
+          rx[s] = load_step<T, V>(xp);
+          rp += a.rt, ip += a.it, xp += a.xt;
+        }
+        const bool reset = SLOW && (z >> s & 1);
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          const float e = decay<SLOW>(r[v], rate[v], reset).e;
+          const float b = feed(i[v], e).ms * x[v];
+          h[v] = reset ? b : fmaf(1.0f - e, h[v], b);
+        }
+        if (at.live) store_step<T, V>(hp, h);
+        hp += a.ht;
+      }
+    };
+    if (big || n < S || __any_sync(0xffffffffu, z != 0)) run(std::true_type{});
+    else run(std::false_type{});
+  }
+  if (a.h_last && at.live) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) a.h_last[at.b * a.D + at.d + v] = h[v];
+  }
+}
+
+// Too few rows and channels for that: blocks of 32 lanes x W warps along time
+// x Z groups of lanes.  A tile is W stretches of S steps: every warp folds its
+// stretch from a zero state in registers to (P, H); the fold threads (one per
+// channel) run through the warps' pairs and give each warp the state before
+// its stretch; every warp then runs its steps again from there and stores
+// them.  In a cluster the blocks take neighbouring tiles and exchange their
+// pairs through distributed shared memory.  One pass over the data; the next
+// tile's loads are in flight during the exchange.
+template <typename T, int V, int S>
+__global__ void __launch_bounds__(256, 2) scan_tile_kernel(const __grid_constant__ ScanArgs a) {
+  __shared__ float2 agg[kWarps][32 * V];
+  __shared__ float pre[kWarps][32 * V];
+  __shared__ float2 cagg[2][kMaxCluster][32 * V];
+  const int lane = threadIdx.x, wt = threadIdx.y, W = blockDim.y;
+  const int slot = threadIdx.z * W;
+  const uint32_t ranks = cluster_size(), rank = cluster_rank();
+  const Place<V> at(a, ((int64_t)(blockIdx.x / ranks) * blockDim.z + threadIdx.z) * 32 + lane);
+  Raw<T, V> rr[S], ri[S], rx[S];
+  auto load = [&](int64_t t0, int n) {
+    const char *r0 = at_step<T>(a.rec, at.b, a.rb, t0, a.rt, at.d);
+    const char *i0 = at_step<T>(a.inp, at.b, a.ib, t0, a.it, at.d);
+    const char *x0 = at_step<T>(a.x, at.b, a.xb, t0, a.xt, at.d);
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      if (s < n) {
+        rr[s] = load_step<T, V>(r0);
+        ri[s] = load_step<T, V>(i0);
+        rx[s] = load_step<T, V>(x0);
+        r0 += a.rt, i0 += a.it, x0 += a.xt;
+      }
+    }
+  };
+  auto steps = [&](int64_t t0) {
+    return (int)max((int64_t)0, min((int64_t)S, a.T - t0));
+  };
+#pragma unroll
+  for (int s = 0; s < S; ++s) rr[s] = ri[s] = rx[s] = Raw<T, V>{};
+  int64_t t0 = ((int64_t)rank * W + wt) * S;
+  int n = steps(t0);
+  load(t0, n);
+  uint32_t z = reset_bits(a, at.b, t0, n, at.one_row);
+  float rate[V], carry[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) carry[v] = a.h0 ? a.h0[at.b * a.D + at.d + v] : 0.0f;
+  const bool big = load_rates<V>(a, at, rate);
   if (ranks > 1) cluster_barrier();  // every block of the cluster runs
 
   int par = 0;
   for (int64_t k0 = 0; k0 < a.tiles; k0 += ranks, par ^= 1) {
-    const int64_t k = k0 + rank, t0 = (k * W + wt) * S;
-    const int n = (int)max((int64_t)0, min((int64_t)S, a.T - t0));
-    Raw<T, V> rr[S], ri[S], rx[S];
-#pragma unroll
-    for (int s = 0; s < S; ++s) {
-      if (s < n) {
-        rr[s] = *reinterpret_cast<const Raw<T, V> *>(rp + (t0 + s) * a.rt);
-        ri[s] = *reinterpret_cast<const Raw<T, V> *>(ip + (t0 + s) * a.it);
-        rx[s] = *reinterpret_cast<const Raw<T, V> *>(xp + (t0 + s) * a.xt);
-      } else {
-        rr[s] = ri[s] = rx[s] = Raw<T, V>{};
-      }
-    }
-    const uint32_t z = n ? reset_bits(a, at.b, t0, n, at.one_row) : 0;
-    const bool slow = big || n < S || __any_sync(0xffffffffu, z != 0);
     float A[S][V], Bv[S][V], P[V], H[V];
     auto fold = [&](auto tag) {
       constexpr bool SLOW = decltype(tag)::value;
@@ -231,279 +341,334 @@ __global__ void __launch_bounds__(256) scan_kernel(const __grid_constant__ ScanA
         const bool reset = SLOW && (z >> s & 1);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-          const Gate g = gate<SLOW>(r[v], i[v], rate[v], reset);
-          A[s][v] = 1.0f - g.e;
-          Bv[s][v] = g.ms * x[v];
+          const float e = decay<SLOW>(r[v], rate[v], reset).e;
+          A[s][v] = 1.0f - e;
+          Bv[s][v] = feed(i[v], e).ms * x[v];
           if (SLOW && s >= n) A[s][v] = 1.0f, Bv[s][v] = 0.0f;
           H[v] = reset ? Bv[s][v] : fmaf(A[s][v], H[v], Bv[s][v]);
           P[v] = reset ? -0.0f : P[v] * A[s][v];
         }
       }
     };
+    const bool slow = big || n < S || __any_sync(0xffffffffu, z != 0);
     if (slow) fold(std::true_type{});
     else fold(std::false_type{});
+    const int64_t t_now = t0;
+    const int n_now = n;
+    const uint32_t z_now = z;
+    t0 += (int64_t)ranks * W * S;
+    n = steps(t0);
+    load(t0, n);
+    z = reset_bits(a, at.b, t0, n, at.one_row);
 
 #pragma unroll
-    for (int v = 0; v < V; ++v) agg[par][slot + wt][v * 32 + lane] = make_float2(P[v], H[v]);
+    for (int v = 0; v < V; ++v) agg[slot + wt][v * 32 + lane] = make_float2(P[v], H[v]);
     __syncthreads();
-    float in[V];
     if (ranks > 1) {
-      // this block's (P, H) to every block, then the blocks before this one
-      float cp[V], ch[V];
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        float2 f = agg[par][slot][v * 32 + lane];
-        cp[v] = f.x, ch[v] = f.y;
+        if (v % W != wt) continue;
+        // this block's (P, H), to every block
+        const int c = v * 32 + lane;
+        float2 f = agg[slot][c];
         for (int w = 1; w < W; ++w) {
-          f = agg[par][slot + w][v * 32 + lane];
-          ch[v] = through(f.x, f.y, ch[v]);
-          cp[v] = __float_as_int(f.x) < 0 ? f.x : f.x * cp[v];
+          const float2 g = agg[slot + w][c];
+          f.y = through(g.x, g.y, f.y);
+          f.x = __float_as_int(g.x) < 0 ? g.x : g.x * f.x;
         }
+        for (uint32_t r = 0; r < ranks; ++r) store_pair_at(&cagg[par][rank][c], r, f);
       }
-      for (uint32_t r = wt; r < ranks; r += W)
-#pragma unroll
-        for (int v = 0; v < V; ++v)
-          store_pair_at(&cagg[par][rank][v * 32 + lane], r, make_float2(cp[v], ch[v]));
       cluster_barrier();
+    }
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
+    for (int v = 0; v < V; ++v) {
+      if (v % W != wt) continue;
+      const int c = v * 32 + lane;
+      float h = carry[v];
+      if (ranks > 1) {
         for (uint32_t r = 0; r < ranks; ++r) {
-          if (r == rank) in[v] = carry[v];
-          const float2 f = cagg[par][r][v * 32 + lane];
+          if (r == rank) h = carry[v];
+          const float2 f = cagg[par][r][c];
           carry[v] = through(f.x, f.y, carry[v]);
         }
       }
-    } else {
-#pragma unroll
-      for (int v = 0; v < V; ++v) in[v] = carry[v];
+      for (int w = 0; w < W; ++w) {
+        pre[slot + w][c] = h;
+        const float2 f = agg[slot + w][c];
+        h = through(f.x, f.y, h);
+      }
+      if (ranks == 1) carry[v] = h;
     }
-    if (a.carry && wt == 0 && k > 0 && n > 0 && at.live) {
-      float *c = a.carry + (at.b * a.K + k - 1) * a.D + at.d;
-#pragma unroll
-      for (int v = 0; v < V; ++v) c[v] = in[v];
-    }
+    __syncthreads();
     float h[V];
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      h[v] = in[v];
-      for (int w = 0; w < W; ++w) {
-        const float2 f = agg[par][slot + w][v * 32 + lane];
-        if (w == wt) h[v] = in[v];
-        in[v] = through(f.x, f.y, in[v]);
-      }
-      if (ranks == 1) carry[v] = in[v];
-    }
-#pragma unroll
-    for (int s = 0; s < S; ++s) {
+    for (int v = 0; v < V; ++v) h[v] = pre[slot + wt][v * 32 + lane];
+    if (a.carry && t_now && n_now && at.live) {
 #pragma unroll
       for (int v = 0; v < V; ++v)
-        h[v] = slow && (z >> s & 1) ? Bv[s][v] : fmaf(A[s][v], h[v], Bv[s][v]);
-      if (s < n && at.live) store_vec<T, V>(hp + (t0 + s) * a.ht, h);
+        a.carry[(at.b * a.K + t_now / kChunk - 1) * a.D + at.d + v] = h[v];
+    }
+    const char *h0 = at_step<T>(a.h, at.b, a.hb, t_now, a.ht, at.d);
+    if (slow) {
+#pragma unroll
+      for (int s = 0; s < S; ++s) {
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+          h[v] = z_now >> s & 1 ? Bv[s][v] : fmaf(A[s][v], h[v], Bv[s][v]);
+        if (s < n_now && at.live) store_step<T, V>(h0, h);
+        h0 += a.ht;
+      }
+    } else {
+#pragma unroll
+      for (int s = 0; s < S; ++s) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) h[v] = fmaf(A[s][v], h[v], Bv[s][v]);
+        if (at.live) store_step<T, V>(h0, h);
+        h0 += a.ht;
+      }
     }
   }
-  if (a.h_last && wt == 0 && rank == 0 && at.live) {
+  if (a.h_last && rank == 0 && at.live) {
 #pragma unroll
-    for (int v = 0; v < V; ++v) a.h_last[at.b * a.D + at.d + v] = carry[v];
+    for (int v = 0; v < V; ++v)
+      if (v % W == wt) a.h_last[at.b * a.D + at.d + v] = carry[v];
   }
 }
 
-// The gradient, tile by tile from the end (the blocks of a cluster take
-// neighbouring tiles, the last first).  A tile's states start from the forward
-// call's carry; the gradient's own recurrence runs backwards with the same P:
-// gamma_t = a_t g_t, g_t = dh_t + gamma_{t+1}.
-template <typename T, int V, int S>
-__global__ void __launch_bounds__(256) scan_grad_kernel(const __grid_constant__ ScanArgs a) {
-  __shared__ float2 agg[2][kWarps][32 * V];  // (P, H)
-  __shared__ float back[2][kWarps][32 * V];  // gamma of a stretch from zero
-  __shared__ float2 cagg[2][kMaxCluster][32 * V];
-  const int lane = threadIdx.x, wt = threadIdx.y, W = blockDim.y;
-  const int slot = threadIdx.z * W;
-  const uint32_t ranks = cluster_size(), rank = cluster_rank();
+// The gradient, stretch by stretch from the end.  Backwards through a stretch,
+// g_t = dh_t + gamma_{t+1}, gamma_t = a_t g_t, from the decays alone; then
+// forwards, with the states running on from the kept one and every output made
+// as its step comes by.  So every gate is computed once and only a, sigmoid(rec)
+// and g of a stretch are held.
+//
+// Rows in one piece (TILED false): a thread takes its channels through all
+// stretches.  Else the warps of a block take the stretches of a tile, and the
+// blocks of a cluster neighbouring tiles, the last first; the pairs (P, gamma
+// from zero) are exchanged as in scan_tile_kernel.
+template <typename T, int V, int S, bool TILED>
+__global__ void __launch_bounds__(256, 2)
+    scan_grad_kernel(const __grid_constant__ ScanArgs a) {
+  __shared__ float2 agg[TILED ? kWarps : 1][32 * V];  // (P, gamma of a stretch from zero)
+  __shared__ float pre[TILED ? kWarps : 1][32 * V];   // gamma after a warp's stretch
+  __shared__ float2 cagg[2][TILED ? kMaxCluster : 1][32 * V];
+  const int lane = threadIdx.x, wt = TILED ? threadIdx.y : 0, W = TILED ? blockDim.y : 1;
+  const int slot = TILED ? threadIdx.z * W : 0;
+  const uint32_t ranks = TILED ? cluster_size() : 1, rank = TILED ? cluster_rank() : 0;
   const Place<V> at(a, ((int64_t)(blockIdx.x / ranks) * blockDim.z + threadIdx.z) * 32 + lane);
-  float rate[V], gam[V], dl[V];
-  bool big = false;
-#pragma unroll
-  for (int v = 0; v < V; ++v) {
-    rate[v] = a.c * softplus(a.lam[at.d + v]);
-    big |= rate[v] > kSeriesMax;
-    gam[v] = a.dh_last ? a.dh_last[at.b * a.D + at.d + v] : 0.0f;
-    dl[v] = 0.0f;
-  }
-  big = __any_sync(0xffffffffu, big);
-  const T *xp = static_cast<const T *>(a.x) + at.b * a.xb + at.d;
-  const T *rp = static_cast<const T *>(a.rec) + at.b * a.rb + at.d;
-  const T *ip = static_cast<const T *>(a.inp) + at.b * a.ib + at.d;
-  const T *gp = static_cast<const T *>(a.dh) + at.b * a.gb + at.d;
-  T *dxp = static_cast<T *>(a.dx) + at.b * a.dxb + at.d;
-  T *drp = static_cast<T *>(a.drec) + at.b * a.drb + at.d;
-  T *dip = static_cast<T *>(a.dinp) + at.b * a.dib + at.d;
-  if (ranks > 1) cluster_barrier();
-
-  int par = 0;
-  for (int64_t k0 = a.tiles - 1; k0 >= 0; k0 -= ranks, par ^= 1) {
-    const int64_t k = k0 - rank, t0 = (k * W + wt) * S;
-    const int n = k < 0 ? 0 : (int)max((int64_t)0, min((int64_t)S, a.T - t0));
-    Raw<T, V> rr[S], ri[S], rx[S], rg[S];
+  Raw<T, V> rr[S], ri[S], rx[S], rg[S];
+  float h[V];
+  auto steps = [&](int64_t t0) {
+    return t0 < 0 ? 0 : (int)max((int64_t)0, min((int64_t)S, a.T - t0));
+  };
+  auto load_back = [&](int64_t t0, int n) {
+    const char *r0 = at_step<T>(a.rec, at.b, a.rb, t0, a.rt, at.d);
+    const char *g0 = at_step<T>(a.dh, at.b, a.gb, t0, a.gt, at.d);
 #pragma unroll
     for (int s = 0; s < S; ++s) {
       if (s < n) {
-        rr[s] = *reinterpret_cast<const Raw<T, V> *>(rp + (t0 + s) * a.rt);
-        ri[s] = *reinterpret_cast<const Raw<T, V> *>(ip + (t0 + s) * a.it);
-        rx[s] = *reinterpret_cast<const Raw<T, V> *>(xp + (t0 + s) * a.xt);
-        rg[s] = *reinterpret_cast<const Raw<T, V> *>(gp + (t0 + s) * a.gt);
-      } else {
-        rr[s] = ri[s] = rx[s] = rg[s] = Raw<T, V>{};
+        rr[s] = load_step<T, V>(r0);
+        rg[s] = load_step<T, V>(g0);
+        r0 += a.rt, g0 += a.gt;
       }
     }
-    float h[V];
+  };
+  auto load_fwd = [&](int64_t t0, int n) {
+    const char *i0 = at_step<T>(a.inp, at.b, a.ib, t0, a.it, at.d);
+    const char *x0 = at_step<T>(a.x, at.b, a.xb, t0, a.xt, at.d);
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      h[v] = 0.0f;
-      if (k > 0) h[v] = a.carry[(at.b * a.K + k - 1) * a.D + at.d + v];
-      else if (k == 0 && a.h0) h[v] = a.h0[at.b * a.D + at.d + v];
+    for (int s = 0; s < S; ++s) {
+      if (s < n) {
+        ri[s] = load_step<T, V>(i0);
+        rx[s] = load_step<T, V>(x0);
+        i0 += a.it, x0 += a.xt;
+      }
     }
-    const uint32_t z = n ? reset_bits(a, at.b, t0, n, at.one_row) : 0;
+    if (n) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        h[v] = 0.0f;
+        if (t0 > 0) h[v] = a.carry[(at.b * a.K + t0 / kChunk - 1) * a.D + at.d + v];
+        else if (a.h0) h[v] = a.h0[at.b * a.D + at.d + v];
+      }
+    }
+  };
+#pragma unroll
+  for (int s = 0; s < S; ++s) rr[s] = ri[s] = rx[s] = rg[s] = Raw<T, V>{};
+#pragma unroll
+  for (int v = 0; v < V; ++v) h[v] = 0.0f;
+  int64_t t0 = ((a.tiles - 1 - rank) * W + wt) * S;
+  int n = steps(t0);
+  load_back(t0, n);
+  load_fwd(t0, n);
+  uint32_t z = reset_bits(a, at.b, t0, n, at.one_row);
+  float rate[V], gam[V], dl[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    gam[v] = a.dh_last ? a.dh_last[at.b * a.D + at.d + v] : 0.0f;
+    dl[v] = 0.0f;
+  }
+  const bool big = load_rates<V>(a, at, rate);
+  if (TILED && ranks > 1) cluster_barrier();
+
+  int par = 0;
+  for (int64_t k0 = a.tiles - 1; k0 >= 0; k0 -= ranks, par ^= 1) {
     const bool slow = big || n < S || __any_sync(0xffffffffu, z != 0);
-    float E[S][V], SR[S][V], MS[S][V], SI[S][V], P[V], H[V], G[V];
-    auto fold = [&](auto tag) {
+    const int64_t t_now = t0;
+    const int n_now = n;
+    const uint32_t z_now = z;
+    float E[S][V], SR[S][V], g[S][V];
+    float P[V], in[V];
+    auto back = [&](auto tag) {
       constexpr bool SLOW = decltype(tag)::value;
 #pragma unroll
-      for (int v = 0; v < V; ++v) P[v] = 1.0f, H[v] = 0.0f, G[v] = 0.0f;
-#pragma unroll
-      for (int s = 0; s < S; ++s) {
-        float r[V], i[V], x[V];
-        unpack<T, V>(rr[s], r);
-        unpack<T, V>(ri[s], i);
-        unpack<T, V>(rx[s], x);
-        const bool reset = SLOW && (z >> s & 1);
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-          const Gate g = gate<SLOW>(r[v], i[v], rate[v], reset);
-          E[s][v] = g.e;
-          SR[s][v] = g.sr;
-          MS[s][v] = g.ms;
-          // sigmoid(inp) = q w^2 s
-          SI[s][v] = g.q * g.w * g.ms;
-          if (SLOW && s >= n) E[s][v] = 0.0f, MS[s][v] = 0.0f;
-          const float A = 1.0f - E[s][v], b = MS[s][v] * x[v];
-          H[v] = reset ? b : fmaf(A, H[v], b);
-          P[v] = reset ? -0.0f : P[v] * A;
-        }
-      }
+      for (int v = 0; v < V; ++v) P[v] = 1.0f, in[v] = 0.0f;
 #pragma unroll
       for (int s = S - 1; s >= 0; --s) {
-        float g[V];
-        unpack<T, V>(rg[s], g);
+        float r[V];
+        unpack<T, V>(rr[s], r);
+        unpack<T, V>(rg[s], g[s]);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-          const float A = 1.0f - E[s][v];
-          G[v] = SLOW && (z >> s & 1) ? 0.0f : A * (G[v] + g[v]);
+          const bool reset = SLOW && (z_now >> s & 1);
+          const Decay q = decay<SLOW>(r[v], rate[v], reset);
+          E[s][v] = q.e;
+          SR[s][v] = q.sr;
+          if (SLOW && s >= n_now) E[s][v] = 0.0f, g[s][v] = 0.0f;
+          if (TILED) {
+            const float A = 1.0f - E[s][v];
+            P[v] = reset ? -0.0f : P[v] * A;
+            in[v] = reset ? 0.0f : A * (in[v] + g[s][v]);
+          }
         }
       }
     };
-    if (slow) fold(std::true_type{});
-    else fold(std::false_type{});
+    if (slow) back(std::true_type{});
+    else back(std::false_type{});
+    t0 -= (int64_t)ranks * W * S;
+    n = steps(t0);
+    load_back(t0, n);
 
+    if (TILED) {
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      agg[par][slot + wt][v * 32 + lane] = make_float2(P[v], H[v]);
-      back[par][slot + wt][v * 32 + lane] = G[v];
-    }
-    __syncthreads();
-    if (ranks > 1) {
-      float cp[V], cg[V];
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        cp[v] = agg[par][slot + W - 1][v * 32 + lane].x;
-        cg[v] = back[par][slot + W - 1][v * 32 + lane];
-        for (int w = W - 2; w >= 0; --w) {
-          const float p = agg[par][slot + w][v * 32 + lane].x;
-          cg[v] = through(p, back[par][slot + w][v * 32 + lane], cg[v]);
-          cp[v] = __float_as_int(p) < 0 ? p : p * cp[v];
-        }
-      }
-      for (uint32_t r = wt; r < ranks; r += W)
-#pragma unroll
-        for (int v = 0; v < V; ++v)
-          store_pair_at(&cagg[par][rank][v * 32 + lane], r, make_float2(cp[v], cg[v]));
-      cluster_barrier();
-    }
-    float g[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      // the state before this warp's steps
-      for (int w = 0; w < wt; ++w) {
-        const float2 f = agg[par][slot + w][v * 32 + lane];
-        h[v] = through(f.x, f.y, h[v]);
-      }
-      // gamma after this warp's steps
-      float in = gam[v];
+      for (int v = 0; v < V; ++v)
+        agg[slot + wt][v * 32 + lane] =
+            make_float2(slow && z_now ? -0.0f : P[v], in[v]);
+      __syncthreads();
       if (ranks > 1) {
-        for (uint32_t r = 0; r < ranks; ++r) {
-          if (r == rank) in = gam[v];
-          const float2 f = cagg[par][r][v * 32 + lane];
-          gam[v] = through(f.x, f.y, gam[v]);
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          if (v % W != wt) continue;
+          const int c = v * 32 + lane;
+          float2 f = agg[slot + W - 1][c];
+          for (int w = W - 2; w >= 0; --w) {
+            const float2 q = agg[slot + w][c];
+            f.y = through(q.x, q.y, f.y);
+            f.x = __float_as_int(q.x) < 0 ? q.x : q.x * f.x;
+          }
+          for (uint32_t r = 0; r < ranks; ++r) store_pair_at(&cagg[par][rank][c], r, f);
+        }
+        cluster_barrier();
+      }
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        if (v % W != wt) continue;
+        const int c = v * 32 + lane;
+        float y = gam[v];
+        if (ranks > 1) {
+          for (uint32_t r = 0; r < ranks; ++r) {
+            if (r == rank) y = gam[v];
+            const float2 f = cagg[par][r][c];
+            gam[v] = through(f.x, f.y, gam[v]);
+          }
+        }
+        for (int w = W - 1; w >= 0; --w) {
+          pre[slot + w][c] = y;
+          const float2 f = agg[slot + w][c];
+          y = through(f.x, f.y, y);
+        }
+        if (ranks == 1) gam[v] = y;
+      }
+      __syncthreads();
+#pragma unroll
+      for (int v = 0; v < V; ++v) in[v] = pre[slot + wt][v * 32 + lane];
+    } else {
+#pragma unroll
+      for (int v = 0; v < V; ++v) in[v] = gam[v];
+    }
+
+    const char *dx0 = at_step<T>(a.dx, at.b, a.dxb, t_now, a.dxt, at.d);
+    const char *dr0 = at_step<T>(a.drec, at.b, a.drb, t_now, a.drt, at.d);
+    const char *di0 = at_step<T>(a.dinp, at.b, a.dib, t_now, a.dit, at.d);
+    auto finish = [&](auto tag) {
+      constexpr bool SLOW = decltype(tag)::value;
+#pragma unroll
+      for (int s = S - 1; s >= 0; --s) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          g[s][v] += in[v];
+          in[v] = SLOW && (z_now >> s & 1) ? 0.0f : (1.0f - E[s][v]) * g[s][v];
         }
       }
-      g[v] = in;
-      for (int w = W - 1; w >= 0; --w) {
-        if (w == wt) g[v] = in;
-        in = through(agg[par][slot + w][v * 32 + lane].x, back[par][slot + w][v * 32 + lane], in);
-      }
-      if (ranks == 1) gam[v] = in;
-    }
-    float before[S][V];
+      if (!TILED) {
 #pragma unroll
-    for (int s = 0; s < S; ++s) {
-      float x[V];
-      unpack<T, V>(rx[s], x);
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        const float b = MS[s][v] * x[v];
-        const bool reset = slow && (z >> s & 1);
-        before[s][v] = reset ? 0.0f : h[v];
-        h[v] = reset ? b : fmaf(1.0f - E[s][v], h[v], b);
+        for (int v = 0; v < V; ++v) gam[v] = in[v];
       }
-    }
 #pragma unroll
-    for (int s = S - 1; s >= 0; --s) {
-      float x[V], d[V], ox[V], orec[V], oinp[V];
-      unpack<T, V>(rx[s], x);
-      unpack<T, V>(rg[s], d);
+      for (int s = 0; s < S; ++s) {
+        if (SLOW && s >= n_now) break;
+        float i[V], x[V], ox[V], orec[V], oinp[V];
+        unpack<T, V>(ri[s], i);
+        unpack<T, V>(rx[s], x);
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        const bool reset = slow && (z >> s & 1);
-        const float e = E[s][v], A = 1.0f - e;
-        const float sq = max_nan(fmaf(-e, e, 2.0f * e), kTinySquare);
-        const float gt = d[v] + g[v];
-        const float gm = gt * MS[s][v];
-        // g (h a - sigmoid(inp) x a^2 / m), and a^2 / m = (m / s) a^2
-        const float q = reset ? 0.0f
-                              : A * (gt * before[s][v] - gm * x[v] * A * rcp(sq));
-        ox[v] = gm;
-        oinp[v] = gm * x[v] * (1.0f - SI[s][v]);
-        const float sq_r = SR[s][v] * q;
-        orec[v] = -rate[v] * (1.0f - SR[s][v]) * sq_r;
-        if (s < n) dl[v] += sq_r;
-        g[v] = reset ? 0.0f : A * gt;
+        for (int v = 0; v < V; ++v) {
+          const bool reset = SLOW && (z_now >> s & 1);
+          const float A = 1.0f - E[s][v];
+          const Feed f = feed(i[v], E[s][v]);
+          const float b = f.ms * x[v];
+          ox[v] = g[s][v] * f.ms;
+          const float gx = ox[v] * x[v];
+          // 1 - sigmoid(inp) = (q - 1) / q and 1 / q = m s_i / m = ms w q
+          const float wq = f.w * f.q;
+          oinp[v] = gx * (1.0f - f.ms * wq);
+          // g (h a - s_i x a^2 / m) = a (g h - g m s_i x a / s), 1 / s = (w q)^2
+          const float q =
+              reset ? 0.0f : A * fmaf(g[s][v], h[v], -(gx * A) * (wq * wq));
+          const float sq = SR[s][v] * q;
+          orec[v] = rate[v] * (SR[s][v] - 1.0f) * sq;
+          dl[v] += sq;
+          h[v] = reset ? b : fmaf(A, h[v], b);
+        }
+        if (at.live) {
+          store_step<T, V>(dx0, ox);
+          store_step<T, V>(dr0, orec);
+          store_step<T, V>(di0, oinp);
+        }
+        dx0 += a.dxt, dr0 += a.drt, di0 += a.dit;
       }
-      if (s < n && at.live) {
-        store_vec<T, V>(dxp + (t0 + s) * a.dxt, ox);
-        store_vec<T, V>(drp + (t0 + s) * a.drt, orec);
-        store_vec<T, V>(dip + (t0 + s) * a.dit, oinp);
-      }
-    }
+    };
+    if (slow) finish(std::true_type{});
+    else finish(std::false_type{});
+    load_fwd(t0, n);
+    z = reset_bits(a, at.b, t0, n, at.one_row);
   }
   // the block's sum for dlam
-  __syncthreads();
+  if (TILED) {
+    __syncthreads();
 #pragma unroll
-  for (int v = 0; v < V; ++v) back[0][slot + wt][v * 32 + lane] = dl[v];
-  __syncthreads();
-  if (wt == 0 && at.live) {
+    for (int v = 0; v < V; ++v) pre[slot + wt][v * 32 + lane] = dl[v];
+    __syncthreads();
+  }
+  if (at.live) {
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      for (int w = 1; w < W; ++w) dl[v] += back[0][slot + w][v * 32 + lane];
-      a.part[((int64_t)rank * a.B + at.b) * a.D + at.d + v] = dl[v];
+      if (v % W != wt) continue;
+      float s = dl[v];
+      if (TILED) {
+        const int c = v * 32 + lane;
+        s = pre[slot][c];
+        for (int w = 1; w < W; ++w) s += pre[slot + w][c];
+      }
+      a.part[((int64_t)rank * a.B + at.b) * a.D + at.d + v] = s;
       if (a.dh0 && rank == 0) a.dh0[at.b * a.D + at.d + v] = gam[v];
     }
   }
@@ -544,11 +709,13 @@ __global__ void __launch_bounds__(1024) scan_dlam_kernel(const float *part, cons
   if (wy == 0 && rank == 0 && d < D) dlam[d] = -c * s / (1.0f + expf(-lam[d]));
 }
 
-// How a call is laid out.  T <= 64: ceil(T / 8) warps cover the whole row, and
-// a block has as many groups of lanes as fit.  Longer rows: 64-step tiles, and
-// where there are too few rows and channels for the SMs, clusters of up to 16
-// blocks that share a row's tiles.
+// How a call is laid out.  Rows in one piece where their channels fill the
+// SMs (or there is one stretch); else tiles: ceil(T / 8) warps cover a row of up
+// to 64 steps, and a block has as many groups of lanes as fit; longer rows go
+// by 64-step tiles, and where there are too few rows and channels for the SMs,
+// clusters of up to 16 blocks share a row's tiles.
 struct ScanPlan {
+  bool rows;
   int V, S, W, Z, ranks;
   int64_t units, tiles, blocks;
 };
@@ -557,14 +724,21 @@ ScanPlan plan_scan(int64_t B, int64_t T, int64_t D, int V) {
   ScanPlan p{};
   p.V = V;
   p.S = T <= 1 ? 1 : kSteps;
-  p.W = (int)std::min<int64_t>(kWarps, std::max<int64_t>(1, (T + p.S - 1) / p.S));
-  p.Z = kWarps / p.W;
   p.units = B * (D / V);
-  p.tiles = (T + p.W * p.S - 1) / (p.W * p.S);
   const int64_t groups = (p.units + 31) / 32;
-  p.Z = (int)std::max<int64_t>(1, std::min<int64_t>(p.Z, groups));
-  const int64_t base = (groups + p.Z - 1) / p.Z;
   p.ranks = 1;
+  p.rows = T <= kSteps || groups >= ROWS_GROUPS;
+  if (p.rows) {
+    p.W = 1;
+    p.tiles = (T + p.S - 1) / p.S;
+    p.Z = kWarps;
+    p.blocks = (groups + p.Z - 1) / p.Z;
+    return p;
+  }
+  p.W = (int)std::min<int64_t>(kWarps, (T + kSteps - 1) / kSteps);
+  p.Z = (int)std::max<int64_t>(1, std::min<int64_t>(kWarps / p.W, groups));
+  p.tiles = (T + p.W * kSteps - 1) / (p.W * kSteps);
+  const int64_t base = (groups + p.Z - 1) / p.Z;
   if (p.Z == 1)
     while (p.ranks < kMaxCluster && base * p.ranks < 2 * 148 && p.tiles >= 2 * p.ranks)
       p.ranks *= 2;
@@ -595,14 +769,29 @@ cudaError_t launch_cluster(K kernel, unsigned blocks, dim3 threads, int ranks, c
 
 int64_t chunk_starts(int64_t T) { return T > 0 ? (T - 1) / kChunk : 0; }
 
-// Whether pairs of channels can be read and written as one access.
-bool pairs_fit(std::initializer_list<const void *> ptrs, const int64_t *strides, int n, int64_t D,
-               int es) {
-  if (D % 2) return false;
-  for (const void *p : ptrs)
-    if (!aligned(p, 2 * es)) return false;
-  for (int i = 0; i < n; ++i)
-    if (strides[i] % 2) return false;
+// A [B, T, D] tensor of a call: where its strides stand in the caller's array
+// and in the kernel's arguments.
+struct ScanTensor {
+  const void *p;
+  int at;
+  int64_t *batch;
+  int32_t *time;
+};
+
+// Fills in the strides; *pairs says whether pairs of channels can be read and
+// written as one access.  False: a time stride does not fit 32 bits of bytes.
+bool place_tensors(ScanTensor *ts, int n, const int64_t *strides, int64_t T, int64_t D, int es,
+                   bool *pairs) {
+  *pairs = D % 2 == 0;
+  for (int i = 0; i < n; ++i) {
+    const int64_t sb = strides ? strides[ts[i].at] : T * D;
+    int64_t st = strides ? strides[ts[i].at + 1] : D;
+    if (T <= 1) st = 0;  // one step: its stride is not used
+    if (st > INT32_MAX / es || st < -(INT32_MAX / es)) return false;
+    *ts[i].batch = sb;
+    *ts[i].time = (int32_t)(st * es);
+    if (sb % 2 || st % 2 || !aligned(ts[i].p, 2 * es)) *pairs = false;
+  }
   return true;
 }
 
@@ -644,12 +833,6 @@ void scan_inputs(ScanArgs &a, const void *x, const void *rec, const void *inp, c
   a.D = D;
   a.K = chunk_starts(T);
   a.c = c;
-  a.xb = strides ? strides[0] : T * D;
-  a.xt = strides ? strides[1] : D;
-  a.rb = strides ? strides[2] : T * D;
-  a.rt = strides ? strides[3] : D;
-  a.ib = strides ? strides[4] : T * D;
-  a.it = strides ? strides[5] : D;
   a.zb = strides ? strides[6] : T;
   a.zt = strides ? strides[7] : 1;
 }
@@ -680,20 +863,29 @@ extern "C" zrl_status zrl_gated_scan(const void *x, const void *rec, const void 
   ScanArgs a{};
   scan_inputs(a, x, rec, inp, lam, h0, resets, B, T, D, c, strides);
   a.h = h;
-  a.hb = strides ? strides[8] : T * D;
-  a.ht = strides ? strides[9] : D;
   a.h_last = h_last;
   a.carry = a.K ? carry : nullptr;
-  const int64_t str[] = {a.xb, a.xt, a.rb, a.rt, a.ib, a.it, a.hb, a.ht};
-  const ScanPlan p = plan_scan(B, T, D, pairs_fit({x, rec, inp, h}, str, 8, D, es) ? 2 : 1);
+  ScanTensor ts[] = {{x, 0, &a.xb, &a.xt}, {rec, 2, &a.rb, &a.rt}, {inp, 4, &a.ib, &a.it},
+                     {h, 8, &a.hb, &a.ht}};
+  bool pairs = false;
+  if (!place_tensors(ts, 4, strides, T, D, es, &pairs))
+    return seq_fail(ZRL_NOT_SUPPORTED, "gated_scan: a time stride of 2 GiB or more");
+  const ScanPlan p = plan_scan(B, T, D, pairs ? 2 : 1);
   if (p.blocks > 0x7fffffff) return seq_fail(ZRL_NOT_SUPPORTED, "gated_scan: B * D too large");
   a.units = p.units;
   a.tiles = p.tiles;
   cudaError_t e = cudaSuccess;
   with_plan(dtype, p, [&](auto t, auto v, auto s) {
-    e = launch_cluster(scan_kernel<decltype(t), decltype(v)::value, decltype(s)::value>,
-                       (unsigned)p.blocks, dim3(32, p.W, p.Z), p.ranks,
-                       static_cast<cudaStream_t>(stream), a);
+    using E = decltype(t);
+    constexpr int V = decltype(v)::value, S = decltype(s)::value;
+    const dim3 threads(32, p.W, p.Z);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (p.rows) {
+      scan_rows_kernel<E, V, S><<<(unsigned)p.blocks, threads, 0, st>>>(a);
+      e = cudaGetLastError();
+    } else if constexpr (S == kSteps) {
+      e = launch_cluster(scan_tile_kernel<E, V, S>, (unsigned)p.blocks, threads, p.ranks, st, a);
+    }
   });
   return scan_launched("gated_scan", e);
 }
@@ -737,19 +929,14 @@ extern "C" zrl_status zrl_gated_scan_grad(
   a.dinp = dinp;
   a.dh0 = dh0;
   a.part = static_cast<float *>(workspace);
-  a.gb = strides ? strides[8] : T * D;
-  a.gt = strides ? strides[9] : D;
-  a.dxb = strides ? strides[10] : T * D;
-  a.dxt = strides ? strides[11] : D;
-  a.drb = strides ? strides[12] : T * D;
-  a.drt = strides ? strides[13] : D;
-  a.dib = strides ? strides[14] : T * D;
-  a.dit = strides ? strides[15] : D;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const int64_t str[] = {a.xb,  a.xt,  a.rb,  a.rt,  a.ib,  a.it,  a.gb,
-                         a.gt,  a.dxb, a.dxt, a.drb, a.drt, a.dib, a.dit};
-  const ScanPlan p =
-      plan_scan(B, T, D, pairs_fit({x, rec, inp, dh, dx, drec, dinp}, str, 14, D, es) ? 2 : 1);
+  ScanTensor ts[] = {{x, 0, &a.xb, &a.xt},     {rec, 2, &a.rb, &a.rt},    {inp, 4, &a.ib, &a.it},
+                     {dh, 8, &a.gb, &a.gt},    {dx, 10, &a.dxb, &a.dxt},  {drec, 12, &a.drb, &a.drt},
+                     {dinp, 14, &a.dib, &a.dit}};
+  bool pairs = false;
+  if (!place_tensors(ts, 7, strides, T, D, es, &pairs))
+    return seq_fail(ZRL_NOT_SUPPORTED, "gated_scan_grad: a time stride of 2 GiB or more");
+  const ScanPlan p = plan_scan(B, T, D, pairs ? 2 : 1);
   if (p.blocks > 0x7fffffff)
     return seq_fail(ZRL_NOT_SUPPORTED, "gated_scan_grad: B * D too large");
   a.units = p.units;
@@ -757,8 +944,16 @@ extern "C" zrl_status zrl_gated_scan_grad(
   cudaError_t e = cudaSuccess;
   if (B)
     with_plan(dtype, p, [&](auto t, auto v, auto s) {
-      e = launch_cluster(scan_grad_kernel<decltype(t), decltype(v)::value, decltype(s)::value>,
-                         (unsigned)p.blocks, dim3(32, p.W, p.Z), p.ranks, st, a);
+      using E = decltype(t);
+      constexpr int V = decltype(v)::value, S = decltype(s)::value;
+      const dim3 threads(32, p.W, p.Z);
+      if (p.rows) {
+        scan_grad_kernel<E, V, S, false><<<(unsigned)p.blocks, threads, 0, st>>>(a);
+        e = cudaGetLastError();
+      } else if constexpr (S == kSteps) {
+        e = launch_cluster(scan_grad_kernel<E, V, S, true>, (unsigned)p.blocks, threads, p.ranks,
+                           st, a);
+      }
     });
   if (e == cudaSuccess) {
     const int64_t rows = B * p.ranks;

@@ -148,7 +148,7 @@ def gated_scan(x, rec, inp, lam, h0=None, resets=None, c: float = 8.0, save: boo
     last = torch.empty((B, D), dtype=torch.float32, device=dev)
     carry = None
     if save:
-        carry = torch.empty((B, max(T - 1, 0) // 64, D), dtype=torch.float32, device=dev)
+        carry = torch.empty((B, max(T - 1, 0) // 8, D), dtype=torch.float32, device=dev)
     st = _strides((("x", x), ("rec", rec), ("inp", inp), ("out", out)), resets)
     _call(N.lib().zrl_gated_scan, dev, x.data_ptr(), rec.data_ptr(), inp.data_ptr(), p_lam,
           p_h0, p_z, B, T, D, dt, c, st, out.data_ptr(), last.data_ptr(),
@@ -197,7 +197,7 @@ def gated_scan_grad(x, rec, inp, lam, dh, carry, dh_last=None, h0=None, resets=N
     B, T, D = shape
     _same("dh", dh, shape, x.dtype, dev)
     p_dl = _f32("dh_last", dh_last, (B, D), dev)
-    p_c = _f32("carry", carry, (B, max(T - 1, 0) // 64, D), dev)
+    p_c = _f32("carry", carry, (B, max(T - 1, 0) // 8, D), dev)
     if out is None:
         out = _like(x), _like(x), _like(x)
     else:
