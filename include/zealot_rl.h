@@ -395,8 +395,8 @@ typedef enum { ZRL_F32 = 0, ZRL_BF16 = 1, ZRL_F16 = 2 } zrl_dtype;
  * h_{-1} = h0 [B, D] (NULL: zeros).  resets [B, T] (bytes, or NULL) marks
  * the steps at which an episode begins; the state before it is not used, not
  * even an infinity or NaN.  x, rec, inp, h: [B, T, D].  h_last [B, D] (or
- * NULL) gets the last state, h0 where T is 0; it may be h0 itself, which is
- * the rollout's single step: T = 1, the state updated in place.  carry (or
+ * NULL) gets the last state, h0 where T is 0; with T = 1 it may be h0 itself,
+ * which is the rollout's step with the state updated in place.  carry (or
  * NULL where no gradient follows) gets zrl_gated_scan_carry() floats: the
  * states before steps 8, 16, ...  strides: (batch, time) of x, rec, inp,
  * resets and h, ten in all.  No counterpart in the reference. */
@@ -404,7 +404,12 @@ zrl_status zrl_gated_scan(const void *x, const void *rec, const void *inp,
                           const float *lam, const float *h0, const uint8_t *resets,
                           int64_t B, int64_t T, int64_t D, int32_t dtype, float c,
                           const int64_t *strides, void *h, float *h_last,
-                          float *carry, void *stream);
+                          float *carry, void *workspace, int64_t workspace_bytes,
+                          void *stream);
+/* Bytes of zrl_gated_scan's workspace (16-byte aligned; 0 where a row is short
+ * or rows and channels alone fill the GPU).  No counterpart in the
+ * reference. */
+int64_t zrl_gated_scan_workspace(int64_t B, int64_t T, int64_t D);
 /* Floats in zrl_gated_scan's carry: B * D for every 8 steps after the
  * first 8.  No counterpart in the reference. */
 int64_t zrl_gated_scan_carry(int64_t B, int64_t T, int64_t D);

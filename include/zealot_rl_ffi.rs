@@ -131,7 +131,9 @@ extern "C" {
     pub fn zrl_gated_scan(x: *const c_void, rec: *const c_void, inp: *const c_void,
                           lam: *const f32, h0: *const f32, resets: *const u8, b: i64, t: i64,
                           d: i64, dtype: i32, c: f32, strides: *const i64, h: *mut c_void,
-                          h_last: *mut f32, carry: *mut f32, stream: *mut c_void) -> c_int;
+                          h_last: *mut f32, carry: *mut f32, workspace: *mut c_void,
+                          workspace_bytes: i64, stream: *mut c_void) -> c_int;
+    pub fn zrl_gated_scan_workspace(b: i64, t: i64, d: i64) -> i64;
     pub fn zrl_gated_scan_carry(b: i64, t: i64, d: i64) -> i64;
     pub fn zrl_gated_scan_grad(x: *const c_void, rec: *const c_void, inp: *const c_void,
                                lam: *const f32, h0: *const f32, resets: *const u8,

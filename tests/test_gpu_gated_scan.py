@@ -375,7 +375,7 @@ def test_refusals_without_a_gpu():
 
     def fwd(b=2, t=3, d=4, dtype=0, c=8.0, x=64, lam=64, h=64):
         return L.zrl_gated_scan(x, 64, 64, lam, None, None, b, t, d, dtype, c, None, h, None,
-                                None, None)
+                                None, None, 0, None)
 
     for kw in (dict(b=-1), dict(t=-1), dict(d=-1), dict(dtype=3), dict(c=0.0), dict(c=-1.0),
                dict(c=float("inf")), dict(x=None), dict(lam=None), dict(h=None), dict(x=66)):

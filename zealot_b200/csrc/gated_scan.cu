@@ -15,8 +15,14 @@
 
 #include "seq_common.cuh"
 
-#ifndef ROWS_GROUPS
-#define ROWS_GROUPS 148 * 16
+#ifndef STEP_BLOCKS
+#define STEP_BLOCKS 148*8
+#endif
+#ifndef SLAB_T
+#define SLAB_T 128
+#endif
+#ifndef SLAB_WARPS
+#define SLAB_WARPS 148*24
 #endif
 namespace zrl {
 namespace {
@@ -24,6 +30,7 @@ namespace {
 constexpr int kSteps = 8;       // steps of a stretch
 constexpr int kWarps = 8;       // warps of a block at most
 constexpr int kMaxCluster = 16;
+constexpr int kMinSlab = 32;    // steps of a slab at least
 // The forward call keeps the state before every stretch after the first; the
 // gradient recomputes the states inside a stretch from there.
 constexpr int kChunk = kSteps;
@@ -37,16 +44,17 @@ struct ScanArgs {
   const uint8_t *resets;
   void *h, *dx, *drec, *dinp;
   float *h_last, *carry, *dh0, *part;
-  int64_t B, T, D, K;   // K: chunk starts after the first
-  int64_t units, tiles; // units of V channels; tiles of one row
+  float2 *fold;         // [slab blocks][B D], then [slabs][B D]
+  int64_t B, T, D, K;   // K: stretches after the first
+  int64_t units;        // units of V channels
+  int64_t slab_steps;   // steps of a slab, a multiple of kSteps (one slab: T or more)
+  int32_t slabs;
   int64_t xb, rb, ib, zb, zt, hb, gb, dxb, drb, dib;  // strides, elements
   int32_t xt, rt, it, ht, gt, dxt, drt, dit;          // strides along time, bytes
   float c;
+  int32_t one;  // 1
 };
 
-__device__ __forceinline__ float softplus(float v) {
-  return fmaxf(v, 0.0f) + log1pf(expf(-fabsf(v)));
-}
 __device__ __forceinline__ float ex2(float v) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
@@ -62,58 +70,160 @@ __device__ __forceinline__ float rsq(float v) {
   asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
   return r;
 }
-// NaN stays NaN, unlike fminf and fmaxf
+// NaN stays NaN, unlike fminf
 __device__ __forceinline__ float min_nan(float a, float b) {
   float r;
   asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
+
+// softplus(v) = max(v, 0) + log(1 + y), y = exp(-|v|), with
+// log(1 + y) = 2 artanh(z), z = y / (2 + y) <= 1/3: its series to z^15 is within
+// 2e-9 relative and keeps the digits of a small y.  7e-7 relative with ex2's
+// and the quotient's roundings; the decays' logarithms scale with it.
+__device__ __forceinline__ float softplus(float v) {
+  const float y = ex2(-fabsf(v) * kLog2e);
+  const float z = y * rcp(2.0f + y), z2 = z * z;
+  float p = fmaf(z2, 1.0f / 15.0f, 1.0f / 13.0f);
+  p = fmaf(z2, p, 1.0f / 11.0f);
+  p = fmaf(z2, p, 1.0f / 9.0f);
+  p = fmaf(z2, p, 1.0f / 7.0f);
+  p = fmaf(z2, p, 1.0f / 5.0f);
+  p = fmaf(z2, p, 1.0f / 3.0f);
+  p = fmaf(z2, p, 1.0f);
+  return (v > 0.0f ? v : v != v ? v : 0.0f) + 2.0f * z * p;
 }
 
-// One element's gates.  With u = rate sigmoid(rec), e = 1 - a = 1 - exp(-u)
+// V channels' values.  Pairs go through the packed fp32 instructions, which
+// halve the issue slots of everything but the special functions.
+template <int V>
+struct Vec {
+  float v[V];
+  __device__ __forceinline__ float &operator[](int i) { return v[i]; }
+  __device__ __forceinline__ const float &operator[](int i) const { return v[i]; }
+};
+template <int V>
+__device__ __forceinline__ Vec<V> all(float c) {
+  Vec<V> r;
+#pragma unroll
+  for (int i = 0; i < V; ++i) r[i] = c;
+  return r;
+}
+template <int V>
+__device__ __forceinline__ Vec<V> fma(const Vec<V> &a, const Vec<V> &b, const Vec<V> &c) {
+  Vec<V> r;
+  if constexpr (V == 2) {
+    const float2 f = __ffma2_rn(make_float2(a[0], a[1]), make_float2(b[0], b[1]),
+                                make_float2(c[0], c[1]));
+    r[0] = f.x, r[1] = f.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) r[i] = fmaf(a[i], b[i], c[i]);
+  }
+  return r;
+}
+template <int V>
+__device__ __forceinline__ Vec<V> mul(const Vec<V> &a, const Vec<V> &b) {
+  Vec<V> r;
+  if constexpr (V == 2) {
+    const float2 f = __fmul2_rn(make_float2(a[0], a[1]), make_float2(b[0], b[1]));
+    r[0] = f.x, r[1] = f.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) r[i] = a[i] * b[i];
+  }
+  return r;
+}
+template <int V>
+__device__ __forceinline__ Vec<V> add(const Vec<V> &a, const Vec<V> &b) {
+  Vec<V> r;
+  if constexpr (V == 2) {
+    const float2 f = __fadd2_rn(make_float2(a[0], a[1]), make_float2(b[0], b[1]));
+    r[0] = f.x, r[1] = f.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) r[i] = a[i] + b[i];
+  }
+  return r;
+}
+template <int V>
+__device__ __forceinline__ Vec<V> fma(const Vec<V> &a, float b, const Vec<V> &c) {
+  return fma(a, all<V>(b), c);
+}
+template <int V>
+__device__ __forceinline__ Vec<V> fma(const Vec<V> &a, const Vec<V> &b, float c) {
+  return fma(a, b, all<V>(c));
+}
+template <int V>
+__device__ __forceinline__ Vec<V> fma(const Vec<V> &a, float b, float c) {
+  return fma(a, all<V>(b), all<V>(c));
+}
+template <int V>
+__device__ __forceinline__ Vec<V> mul(const Vec<V> &a, float b) {
+  return mul(a, all<V>(b));
+}
+template <int V>
+__device__ __forceinline__ Vec<V> add(const Vec<V> &a, float b) {
+  return add(a, all<V>(b));
+}
+
+// The gates of one step.  With u = rate sigmoid(rec), e = 1 - a = 1 - exp(-u)
 // comes from its series up to u = 0.35 (seven terms, 2e-8 relative): a = 1 - e
 // is then within half a unit of exp(-u) at every step, so the roundings of a
 // long memory do not add up in one direction, and s = 1 - a^2 = e (2 - e)
 // keeps its digits where a is near 1.  Above (only SLOW looks), a comes from
-// ex2.  exp(-rec) is held to 2^126 and s to at least 2^-120, so nothing
-// overflows or divides by zero.
+// ex2.  exp(-rec) may be infinite: sigmoid(rec) and e are then 0.
+template <int V>
 struct Decay {
-  float sr, e;  // sigmoid(rec), 1 - a
+  Vec<V> sr, e, a;  // sigmoid(rec), 1 - a, a
 };
-template <bool SLOW>
-__device__ __forceinline__ Decay decay(float rec, float rate, bool reset) {
-  Decay g;
-  g.sr = rcp(1.0f + ex2(min_nan(rec * -kLog2e, 126.0f)));
-  const float u = rate * g.sr;
-  float p = fmaf(u, 1.0f / 5040.0f, -1.0f / 720.0f);
-  p = fmaf(u, p, 1.0f / 120.0f);
-  p = fmaf(u, p, -1.0f / 24.0f);
-  p = fmaf(u, p, 1.0f / 6.0f);
-  p = fmaf(u, p, -0.5f);
-  p = fmaf(u, p, 1.0f);
-  g.e = u * p;
+template <bool SLOW, int V>
+__device__ __forceinline__ Decay<V> decay(const Vec<V> &rec, const Vec<V> &rate, bool reset) {
+  Decay<V> g;
+  Vec<V> t = mul(rec, -kLog2e);
+#pragma unroll
+  for (int v = 0; v < V; ++v) t[v] = ex2(t[v]);
+  t = add(t, 1.0f);
+#pragma unroll
+  for (int v = 0; v < V; ++v) g.sr[v] = rcp(t[v]);
+  const Vec<V> u = mul(rate, g.sr);
+  Vec<V> p = fma(u, 1.0f / 5040.0f, -1.0f / 720.0f);
+  p = fma(u, p, 1.0f / 120.0f);
+  p = fma(u, p, -1.0f / 24.0f);
+  p = fma(u, p, 1.0f / 6.0f);
+  p = fma(u, p, -0.5f);
+  p = fma(u, p, 1.0f);
+  g.e = mul(u, p);
   if (SLOW) {
-    if (u > kSeriesMax) g.e = 1.0f - ex2(u * -kLog2e);
-    if (reset) g.e = 1.0f;  // a = 0, m = 1
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      if (u[v] > kSeriesMax) g.e[v] = 1.0f - ex2(u[v] * -kLog2e);
+      if (reset) g.e[v] = 1.0f;  // a = 0, m = 1
+    }
   }
+  g.a = fma(g.e, -1.0f, 1.0f);
   return g;
 }
 // m sigmoid(inp) = s w with w = 1 / sqrt(s q^2), q = 1 + exp(-inp): one
-// reciprocal square root for the square root and the quotient.  exp(-inp) is
-// held to 2^60.
+// reciprocal square root for the square root and the quotient.  2^-120 on s
+// keeps w finite where a is 1; q may be infinite (w and m sigmoid(inp) are then
+// 0) unless HELD, which holds it to 2^60 for the products of w and q.
+template <int V>
 struct Feed {
-  float ms, w, q;
+  Vec<V> ms, w, q;
 };
-__device__ __forceinline__ Feed feed(float inp, float e) {
-  Feed f;
-  f.q = 1.0f + ex2(min_nan(inp * -kLog2e, 60.0f));
-  const float s = max_nan(fmaf(-e, e, 2.0f * e), kTinySquare);
-  f.w = rsq(s * f.q * f.q);
-  f.ms = s * f.w;
+template <bool HELD, int V>
+__device__ __forceinline__ Feed<V> feed(const Vec<V> &inp, const Vec<V> &e, const Vec<V> &a) {
+  Feed<V> f;
+  Vec<V> t = mul(inp, -kLog2e);
+#pragma unroll
+  for (int v = 0; v < V; ++v) t[v] = ex2(HELD ? min_nan(t[v], 60.0f) : t[v]);
+  f.q = add(t, 1.0f);
+  const Vec<V> s = fma(e, add(a, 1.0f), kTinySquare);
+  t = mul(mul(s, f.q), f.q);
+#pragma unroll
+  for (int v = 0; v < V; ++v) f.w[v] = rsq(t[v]);
+  f.ms = mul(s, f.w);
   return f;
 }
 
@@ -154,30 +264,41 @@ __device__ __forceinline__ const char *at_step(const void *p, int64_t b, int64_t
   return static_cast<const char *>(p) + (b * sb + d) * (int64_t)sizeof(T) + t * st;
 }
 template <typename T, int V>
+__device__ __forceinline__ Vec<V> values(const Raw<T, V> &raw) {
+  Vec<V> r;
+  unpack<T, V>(raw, r.v);
+  return r;
+}
+template <typename T, int V>
 __device__ __forceinline__ Raw<T, V> load_step(const char *p) {
   return *reinterpret_cast<const Raw<T, V> *>(p);
 }
 template <typename T, int V>
-__device__ __forceinline__ void store_step(const char *p, const float *v) {
-  *reinterpret_cast<Raw<T, V> *>(const_cast<char *>(p)) = pack<T, V>(v);
+__device__ __forceinline__ void store_step(const char *p, const Vec<V> &x) {
+  *reinterpret_cast<Raw<T, V> *>(const_cast<char *>(p)) = pack<T, V>(x.v);
 }
 
-// The reset marks of steps t .. t + n - 1 of the lane's row, bit s for step s.
-// A warp whose lanes share a row reads each mark once.
-__device__ __forceinline__ uint32_t reset_bits(const ScanArgs &a, int64_t b, int64_t t, int n,
+// p + stride as one multiply-add (one is 1, which the compiler cannot know).
+__device__ __forceinline__ void advance(const char *&p, int32_t stride, int32_t one) {
+  asm("mad.wide.s32 %0, %1, %2, %0;" : "+l"(p) : "r"(stride), "r"(one));
+}
+
+// The reset marks of steps t .. t + n - 1 of the lane's row, to be turned into
+// bits (bit s for step s) where they are needed, so that their latency is not
+// waited for.  A warp whose lanes share a row reads each mark once.
+__device__ __forceinline__ uint32_t load_marks(const ScanArgs &a, int64_t b, int64_t t, int n,
                                                bool one_row) {
   if (!a.resets) return 0;
   const uint8_t *z = a.resets + b * a.zb + t * a.zt;
+  if (one_row) return (int)threadIdx.x < n ? z[threadIdx.x * a.zt] : 0;
   uint32_t bits = 0;
-  if (one_row) {
-    const int lane = threadIdx.x;
-    const bool on = lane < n && z[lane * a.zt];
-    bits = __ballot_sync(0xffffffffu, on);
-  } else {
 #pragma unroll 1
-    for (int s = 0; s < n; ++s) bits |= (z[s * a.zt] ? 1u : 0u) << s;
-  }
+  for (int s = 0; s < n; ++s) bits |= (z[s * a.zt] ? 1u : 0u) << s;
   return bits;
+}
+__device__ __forceinline__ uint32_t mark_bits(const ScanArgs &a, uint32_t marks, bool one_row) {
+  if (!a.resets) return 0;
+  return one_row ? __ballot_sync(0xffffffffu, marks != 0) : marks;
 }
 
 // Which channels a lane has: V of them from d in row b.
@@ -200,7 +321,7 @@ struct Place {
 };
 
 template <int V>
-__device__ __forceinline__ bool load_rates(const ScanArgs &a, const Place<V> &at, float *rate) {
+__device__ __forceinline__ bool load_rates(const ScanArgs &a, const Place<V> &at, Vec<V> &rate) {
   bool big = false;
 #pragma unroll
   for (int v = 0; v < V; ++v) {
@@ -210,255 +331,241 @@ __device__ __forceinline__ bool load_rates(const ScanArgs &a, const Place<V> &at
   return __any_sync(0xffffffffu, big);
 }
 
-// Rows in one piece: a thread takes its V channels through all steps, with the
-// loads of the S steps ahead in flight.
-template <typename T, int V, int S>
-__global__ void __launch_bounds__(256) scan_rows_kernel(const __grid_constant__ ScanArgs a) {
-  const Place<V> at(a, ((int64_t)blockIdx.x * blockDim.z + threadIdx.z) * 32 + threadIdx.x);
+// Blocks of 32 lanes x 8 warps.  One slab: the warps take neighbouring groups of
+// lanes.  Several: they take neighbouring slabs of one group.
+struct Slab {
+  int64_t group, begin, end;
+  int32_t index;
+  __device__ __forceinline__ explicit Slab(const ScanArgs &a) {
+    if (a.slabs == 1) {
+      group = (int64_t)blockIdx.x * kWarps + threadIdx.y;
+      index = 0;
+    } else {
+      group = blockIdx.x;
+      index = blockIdx.y * kWarps + threadIdx.y;
+    }
+    begin = index * a.slab_steps;
+    end = min(a.T, begin + a.slab_steps);
+  }
+};
+
+// What a slab does to the state before it (BACK: to the gradient after it), as a
+// pair (P, H): every warp folds its slab, then the block writes, per warp, the
+// pair of the block's slabs before (after) it, and the pair of them all.
+template <typename T, int V, bool BACK>
+__global__ void __launch_bounds__(256) scan_fold_kernel(const __grid_constant__ ScanArgs a) {
+  constexpr int S = kSteps;
+  __shared__ float2 agg[kWarps][32 * V];
+  const int lane = threadIdx.x, wt = threadIdx.y;
+  const Slab slab(a);
+  const Place<V> at(a, slab.group * 32 + lane);
+  const int64_t steps = max((int64_t)0, slab.end - slab.begin);
+  // in the order of the recurrence: forward from begin, or back from end - 1
+  const int dir = BACK ? -1 : 1;
+  const int64_t first = BACK ? slab.end - 1 : slab.begin;
+  const char *rp = at_step<T>(a.rec, at.b, a.rb, first, a.rt, at.d);
+  const char *ip = BACK ? at_step<T>(a.dh, at.b, a.gb, first, a.gt, at.d)
+                        : at_step<T>(a.inp, at.b, a.ib, first, a.it, at.d);
+  const char *xp = at_step<T>(a.x, at.b, a.xb, first, a.xt, at.d);
+  const int32_t rt = dir * a.rt, it = BACK ? -a.gt : a.it, xt = a.xt;
   Raw<T, V> rr[S], ri[S], rx[S];
-  const char *rp = at_step<T>(a.rec, at.b, a.rb, 0, a.rt, at.d);
-  const char *ip = at_step<T>(a.inp, at.b, a.ib, 0, a.it, at.d);
-  const char *xp = at_step<T>(a.x, at.b, a.xb, 0, a.xt, at.d);
 #pragma unroll
   for (int s = 0; s < S; ++s) {
     rr[s] = ri[s] = rx[s] = Raw<T, V>{};
-    if (s < a.T) {
+    if (s < steps) {
+      rr[s] = load_step<T, V>(rp);
+      ri[s] = load_step<T, V>(ip);
+      if (!BACK) rx[s] = load_step<T, V>(xp);
+    }
+    advance(rp, rt, a.one);
+    advance(ip, it, a.one);
+    if (!BACK) advance(xp, xt, a.one);
+  }
+  Vec<V> rate;
+  const bool big = load_rates<V>(a, at, rate);
+  Vec<V> P = all<V>(1.0f), H = all<V>(0.0f);
+  // marks of the n steps that follow done steps, bit s for the lowest step
+  auto marks_of = [&](int64_t done, int n) {
+    return load_marks(a, at.b, BACK ? slab.end - done - n : slab.begin + done, n, at.one_row);
+  };
+  uint32_t marks = marks_of(0, (int)min((int64_t)S, steps));
+  for (int64_t t = 0; t < steps; t += S) {
+    const int n = (int)min((int64_t)S, steps - t);
+    const int ahead = (int)max((int64_t)0, min((int64_t)S, steps - t - S));
+    const uint32_t z = mark_bits(a, marks, at.one_row);
+    marks = marks_of(t + S, ahead);
+    auto run = [&](auto slow, auto more) {
+      constexpr bool SLOW = decltype(slow)::value, MORE = decltype(more)::value;
+#pragma unroll
+      for (int s = 0; s < S; ++s) {
+        if (SLOW && s >= n) break;
+        const Vec<V> r = values<T, V>(rr[s]), i = values<T, V>(ri[s]), x = values<T, V>(rx[s]);
+        if (MORE || (SLOW && s < ahead)) {
+          rr[s] = load_step<T, V>(rp);
+          ri[s] = load_step<T, V>(ip);
+          if (!BACK) rx[s] = load_step<T, V>(xp);
+          advance(rp, rt, a.one);
+          advance(ip, it, a.one);
+          if (!BACK) advance(xp, xt, a.one);
+        }
+        const bool reset = SLOW && (z >> (BACK ? n - 1 - s : s) & 1);
+        const Decay<V> g = decay<SLOW>(r, rate, reset);
+        if (BACK) {
+          H = mul(g.a, add(H, i));
+          if (reset) H = all<V>(0.0f);
+        } else {
+          const Vec<V> b = mul(feed<false>(i, g.e, g.a).ms, x);
+          if (reset) H = b;
+          else H = fma(g.a, H, b);
+        }
+        if (reset) P = all<V>(-0.0f);
+        else P = mul(P, g.a);
+      }
+    };
+    if (big || n < S || (ahead != 0 && ahead != S) || __any_sync(0xffffffffu, z != 0))
+      run(std::true_type{}, std::false_type{});
+    else if (ahead)
+      run(std::false_type{}, std::true_type{});
+    else
+      run(std::false_type{}, std::false_type{});
+  }
+#pragma unroll
+  for (int v = 0; v < V; ++v) agg[wt][v * 32 + lane] = make_float2(P[v], H[v]);
+  __syncthreads();
+  if (!at.live) return;
+  float2 *whole = a.fold + (int64_t)blockIdx.y * a.B * a.D;
+  float2 *own = a.fold + ((int64_t)gridDim.y + slab.index) * a.B * a.D;
+  const int64_t c = at.b * a.D + at.d;
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    float2 f = make_float2(1.0f, 0.0f);
+    for (int i = 0; i < kWarps; ++i) {
+      const int w = BACK ? kWarps - 1 - i : i;
+      if (w == wt) own[c + v] = f;
+      const float2 g = agg[w][v * 32 + lane];
+      f.y = through(g.x, g.y, f.y);
+      f.x = __float_as_int(g.x) < 0 ? g.x : g.x * f.x;
+    }
+    if (wt == 0) whole[c + v] = f;
+  }
+}
+
+// The state before a slab (BACK: the gradient after it) from first, the state
+// before the row (the gradient after it): through the blocks of slabs, then
+// the slabs of its own block.
+template <bool BACK, int V>
+__device__ __forceinline__ void enter_slab(const ScanArgs &a, const Slab &slab, const Place<V> &at,
+                                           Vec<V> &h) {
+  if (a.slabs == 1) return;
+  const int64_t c = at.b * a.D + at.d, row = a.B * a.D;
+  const int blocks = gridDim.y, mine = blockIdx.y;
+#pragma unroll 8
+  for (int i = 0; i < (BACK ? blocks - 1 - mine : mine); ++i) {
+    const float2 *f = a.fold + (BACK ? blocks - 1 - i : i) * row + c;
+#pragma unroll
+    for (int v = 0; v < V; ++v) h[v] = through(f[v].x, f[v].y, h[v]);
+  }
+  const float2 *f = a.fold + (blocks + slab.index) * row + c;
+#pragma unroll
+  for (int v = 0; v < V; ++v) h[v] = through(f[v].x, f[v].y, h[v]);
+}
+
+// A thread takes its V channels through the steps of its slab, with the loads
+// of the eight steps ahead in flight.
+template <typename T, int V>
+__global__ void __launch_bounds__(256) scan_kernel(const __grid_constant__ ScanArgs a) {
+  constexpr int S = kSteps;
+  const Slab slab(a);
+  const Place<V> at(a, slab.group * 32 + threadIdx.x);
+  if (!__any_sync(0xffffffffu, at.live)) return;
+  const char *rp = at_step<T>(a.rec, at.b, a.rb, slab.begin, a.rt, at.d);
+  const char *ip = at_step<T>(a.inp, at.b, a.ib, slab.begin, a.it, at.d);
+  const char *xp = at_step<T>(a.x, at.b, a.xb, slab.begin, a.xt, at.d);
+  Raw<T, V> rr[S], ri[S], rx[S];
+#pragma unroll
+  for (int s = 0; s < S; ++s) {
+    rr[s] = ri[s] = rx[s] = Raw<T, V>{};
+    if (slab.begin + s < slab.end) {
       rr[s] = load_step<T, V>(rp);
       ri[s] = load_step<T, V>(ip);
       rx[s] = load_step<T, V>(xp);
     }
-    rp += a.rt, ip += a.it, xp += a.xt;
+    advance(rp, a.rt, a.one);
+    advance(ip, a.it, a.one);
+    advance(xp, a.xt, a.one);
   }
-  float h[V], rate[V];
+  auto count = [&](int64_t t) {
+    return (int)max((int64_t)0, min((int64_t)S, slab.end - t));
+  };
+  uint32_t marks = load_marks(a, at.b, slab.begin, count(slab.begin), at.one_row);
+  Vec<V> h, rate;
 #pragma unroll
   for (int v = 0; v < V; ++v) h[v] = a.h0 ? a.h0[at.b * a.D + at.d + v] : 0.0f;
+  enter_slab<false>(a, slab, at, h);
   const bool big = load_rates<V>(a, at, rate);
-  const char *hp = at_step<T>(a.h, at.b, a.hb, 0, a.ht, at.d);
-  for (int64_t t0 = 0; t0 < a.T; t0 += S) {
-    const int n = (int)min((int64_t)S, a.T - t0);
-    const int ahead = (int)max((int64_t)0, min((int64_t)S, a.T - t0 - S));
-    const uint32_t z = reset_bits(a, at.b, t0, n, at.one_row);
-    if (a.carry && t0 && at.live) {
+  const char *hp = at_step<T>(a.h, at.b, a.hb, slab.begin, a.ht, at.d);
+  for (int64_t t0 = slab.begin; t0 < slab.end; t0 += S) {
+    const int n = count(t0), ahead = count(t0 + S);
+    const uint32_t z = mark_bits(a, marks, at.one_row);
+    marks = load_marks(a, at.b, t0 + S, ahead, at.one_row);
+    if (a.carry && t0) {
 #pragma unroll
       for (int v = 0; v < V; ++v)
         a.carry[(at.b * a.K + t0 / kChunk - 1) * a.D + at.d + v] = h[v];
     }
-    auto run = [&](auto tag) {
-      constexpr bool SLOW = decltype(tag)::value;
+    // A lane beyond the last channel repeats the last one's steps and stores.
+    auto run = [&](auto slow, auto more) {
+      constexpr bool SLOW = decltype(slow)::value, MORE = decltype(more)::value;
 #pragma unroll
       for (int s = 0; s < S; ++s) {
         if (SLOW && s >= n) break;
-        float r[V], i[V], x[V];
-        unpack<T, V>(rr[s], r);
-        unpack<T, V>(ri[s], i);
-        unpack<T, V>(rx[s], x);
-        if (s < ahead) {
+        const Vec<V> r = values<T, V>(rr[s]), i = values<T, V>(ri[s]), x = values<T, V>(rx[s]);
+        if (MORE || (SLOW && s < ahead)) {
           rr[s] = load_step<T, V>(rp);
           ri[s] = load_step<T, V>(ip);
           rx[s] = load_step<T, V>(xp);
-          rp += a.rt, ip += a.it, xp += a.xt;
+          advance(rp, a.rt, a.one);
+          advance(ip, a.it, a.one);
+          advance(xp, a.xt, a.one);
         }
         const bool reset = SLOW && (z >> s & 1);
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-          const float e = decay<SLOW>(r[v], rate[v], reset).e;
-          const float b = feed(i[v], e).ms * x[v];
-          h[v] = reset ? b : fmaf(1.0f - e, h[v], b);
-        }
-        if (at.live) store_step<T, V>(hp, h);
-        hp += a.ht;
+        const Decay<V> g = decay<SLOW>(r, rate, reset);
+        const Vec<V> b = mul(feed<false>(i, g.e, g.a).ms, x);
+        if (reset) h = b;
+        else h = fma(g.a, h, b);
+        store_step<T, V>(hp, h);
+        advance(hp, a.ht, a.one);
       }
     };
-    if (big || n < S || __any_sync(0xffffffffu, z != 0)) run(std::true_type{});
-    else run(std::false_type{});
+    if (big || n < S || (ahead != 0 && ahead != S) || __any_sync(0xffffffffu, z != 0))
+      run(std::true_type{}, std::false_type{});
+    else if (ahead)
+      run(std::false_type{}, std::true_type{});
+    else
+      run(std::false_type{}, std::false_type{});
   }
-  if (a.h_last && at.live) {
+  if (a.h_last && slab.index == a.slabs - 1) {
 #pragma unroll
     for (int v = 0; v < V; ++v) a.h_last[at.b * a.D + at.d + v] = h[v];
   }
 }
 
-// Too few rows and channels for that: blocks of 32 lanes x W warps along time
-// x Z groups of lanes.  A tile is W stretches of S steps: every warp folds its
-// stretch from a zero state in registers to (P, H); the fold threads (one per
-// channel) run through the warps' pairs and give each warp the state before
-// its stretch; every warp then runs its steps again from there and stores
-// them.  In a cluster the blocks take neighbouring tiles and exchange their
-// pairs through distributed shared memory.  One pass over the data; the next
-// tile's loads are in flight during the exchange.
-template <typename T, int V, int S>
-__global__ void __launch_bounds__(256, 2) scan_tile_kernel(const __grid_constant__ ScanArgs a) {
-  __shared__ float2 agg[kWarps][32 * V];
-  __shared__ float pre[kWarps][32 * V];
-  __shared__ float2 cagg[2][kMaxCluster][32 * V];
-  const int lane = threadIdx.x, wt = threadIdx.y, W = blockDim.y;
-  const int slot = threadIdx.z * W;
-  const uint32_t ranks = cluster_size(), rank = cluster_rank();
-  const Place<V> at(a, ((int64_t)(blockIdx.x / ranks) * blockDim.z + threadIdx.z) * 32 + lane);
-  Raw<T, V> rr[S], ri[S], rx[S];
-  auto load = [&](int64_t t0, int n) {
-    const char *r0 = at_step<T>(a.rec, at.b, a.rb, t0, a.rt, at.d);
-    const char *i0 = at_step<T>(a.inp, at.b, a.ib, t0, a.it, at.d);
-    const char *x0 = at_step<T>(a.x, at.b, a.xb, t0, a.xt, at.d);
-#pragma unroll
-    for (int s = 0; s < S; ++s) {
-      if (s < n) {
-        rr[s] = load_step<T, V>(r0);
-        ri[s] = load_step<T, V>(i0);
-        rx[s] = load_step<T, V>(x0);
-        r0 += a.rt, i0 += a.it, x0 += a.xt;
-      }
-    }
-  };
-  auto steps = [&](int64_t t0) {
-    return (int)max((int64_t)0, min((int64_t)S, a.T - t0));
-  };
-#pragma unroll
-  for (int s = 0; s < S; ++s) rr[s] = ri[s] = rx[s] = Raw<T, V>{};
-  int64_t t0 = ((int64_t)rank * W + wt) * S;
-  int n = steps(t0);
-  load(t0, n);
-  uint32_t z = reset_bits(a, at.b, t0, n, at.one_row);
-  float rate[V], carry[V];
-#pragma unroll
-  for (int v = 0; v < V; ++v) carry[v] = a.h0 ? a.h0[at.b * a.D + at.d + v] : 0.0f;
-  const bool big = load_rates<V>(a, at, rate);
-  if (ranks > 1) cluster_barrier();  // every block of the cluster runs
-
-  int par = 0;
-  for (int64_t k0 = 0; k0 < a.tiles; k0 += ranks, par ^= 1) {
-    float A[S][V], Bv[S][V], P[V], H[V];
-    auto fold = [&](auto tag) {
-      constexpr bool SLOW = decltype(tag)::value;
-#pragma unroll
-      for (int v = 0; v < V; ++v) P[v] = 1.0f, H[v] = 0.0f;
-#pragma unroll
-      for (int s = 0; s < S; ++s) {
-        float r[V], i[V], x[V];
-        unpack<T, V>(rr[s], r);
-        unpack<T, V>(ri[s], i);
-        unpack<T, V>(rx[s], x);
-        const bool reset = SLOW && (z >> s & 1);
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-          const float e = decay<SLOW>(r[v], rate[v], reset).e;
-          A[s][v] = 1.0f - e;
-          Bv[s][v] = feed(i[v], e).ms * x[v];
-          if (SLOW && s >= n) A[s][v] = 1.0f, Bv[s][v] = 0.0f;
-          H[v] = reset ? Bv[s][v] : fmaf(A[s][v], H[v], Bv[s][v]);
-          P[v] = reset ? -0.0f : P[v] * A[s][v];
-        }
-      }
-    };
-    const bool slow = big || n < S || __any_sync(0xffffffffu, z != 0);
-    if (slow) fold(std::true_type{});
-    else fold(std::false_type{});
-    const int64_t t_now = t0;
-    const int n_now = n;
-    const uint32_t z_now = z;
-    t0 += (int64_t)ranks * W * S;
-    n = steps(t0);
-    load(t0, n);
-    z = reset_bits(a, at.b, t0, n, at.one_row);
-
-#pragma unroll
-    for (int v = 0; v < V; ++v) agg[slot + wt][v * 32 + lane] = make_float2(P[v], H[v]);
-    __syncthreads();
-    if (ranks > 1) {
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        if (v % W != wt) continue;
-        // this block's (P, H), to every block
-        const int c = v * 32 + lane;
-        float2 f = agg[slot][c];
-        for (int w = 1; w < W; ++w) {
-          const float2 g = agg[slot + w][c];
-          f.y = through(g.x, g.y, f.y);
-          f.x = __float_as_int(g.x) < 0 ? g.x : g.x * f.x;
-        }
-        for (uint32_t r = 0; r < ranks; ++r) store_pair_at(&cagg[par][rank][c], r, f);
-      }
-      cluster_barrier();
-    }
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      if (v % W != wt) continue;
-      const int c = v * 32 + lane;
-      float h = carry[v];
-      if (ranks > 1) {
-        for (uint32_t r = 0; r < ranks; ++r) {
-          if (r == rank) h = carry[v];
-          const float2 f = cagg[par][r][c];
-          carry[v] = through(f.x, f.y, carry[v]);
-        }
-      }
-      for (int w = 0; w < W; ++w) {
-        pre[slot + w][c] = h;
-        const float2 f = agg[slot + w][c];
-        h = through(f.x, f.y, h);
-      }
-      if (ranks == 1) carry[v] = h;
-    }
-    __syncthreads();
-    float h[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) h[v] = pre[slot + wt][v * 32 + lane];
-    if (a.carry && t_now && n_now && at.live) {
-#pragma unroll
-      for (int v = 0; v < V; ++v)
-        a.carry[(at.b * a.K + t_now / kChunk - 1) * a.D + at.d + v] = h[v];
-    }
-    const char *h0 = at_step<T>(a.h, at.b, a.hb, t_now, a.ht, at.d);
-    if (slow) {
-#pragma unroll
-      for (int s = 0; s < S; ++s) {
-#pragma unroll
-        for (int v = 0; v < V; ++v)
-          h[v] = z_now >> s & 1 ? Bv[s][v] : fmaf(A[s][v], h[v], Bv[s][v]);
-        if (s < n_now && at.live) store_step<T, V>(h0, h);
-        h0 += a.ht;
-      }
-    } else {
-#pragma unroll
-      for (int s = 0; s < S; ++s) {
-#pragma unroll
-        for (int v = 0; v < V; ++v) h[v] = fmaf(A[s][v], h[v], Bv[s][v]);
-        if (at.live) store_step<T, V>(h0, h);
-        h0 += a.ht;
-      }
-    }
-  }
-  if (a.h_last && rank == 0 && at.live) {
-#pragma unroll
-    for (int v = 0; v < V; ++v)
-      if (v % W == wt) a.h_last[at.b * a.D + at.d + v] = carry[v];
-  }
-}
-
-// The gradient, stretch by stretch from the end.  Backwards through a stretch,
-// g_t = dh_t + gamma_{t+1}, gamma_t = a_t g_t, from the decays alone; then
-// forwards, with the states running on from the kept one and every output made
-// as its step comes by.  So every gate is computed once and only a, sigmoid(rec)
-// and g of a stretch are held.
-//
-// Rows in one piece (TILED false): a thread takes its channels through all
-// stretches.  Else the warps of a block take the stretches of a tile, and the
-// blocks of a cluster neighbouring tiles, the last first; the pairs (P, gamma
-// from zero) are exchanged as in scan_tile_kernel.
-template <typename T, int V, int S, bool TILED>
+// The gradient, stretch by stretch from a slab's end.  Backwards through a
+// stretch, g_t = dh_t + gamma_{t+1}, gamma_t = a_t g_t, from the decays alone;
+// then forwards, with the states running on from the kept one and every output
+// made as its step comes by.  So every gate is computed once and only 1 - a,
+// sigmoid(rec) and g of a stretch are held.
+template <typename T, int V>
 __global__ void __launch_bounds__(256, 2)
     scan_grad_kernel(const __grid_constant__ ScanArgs a) {
-  __shared__ float2 agg[TILED ? kWarps : 1][32 * V];  // (P, gamma of a stretch from zero)
-  __shared__ float pre[TILED ? kWarps : 1][32 * V];   // gamma after a warp's stretch
-  __shared__ float2 cagg[2][TILED ? kMaxCluster : 1][32 * V];
-  const int lane = threadIdx.x, wt = TILED ? threadIdx.y : 0, W = TILED ? blockDim.y : 1;
-  const int slot = TILED ? threadIdx.z * W : 0;
-  const uint32_t ranks = TILED ? cluster_size() : 1, rank = TILED ? cluster_rank() : 0;
-  const Place<V> at(a, ((int64_t)(blockIdx.x / ranks) * blockDim.z + threadIdx.z) * 32 + lane);
+  constexpr int S = kSteps;
+  const Slab slab(a);
+  const Place<V> at(a, slab.group * 32 + threadIdx.x);
+  if (!__any_sync(0xffffffffu, at.live)) return;
   Raw<T, V> rr[S], ri[S], rx[S], rg[S];
-  float h[V];
-  auto steps = [&](int64_t t0) {
-    return t0 < 0 ? 0 : (int)max((int64_t)0, min((int64_t)S, a.T - t0));
+  Vec<V> h = all<V>(0.0f);
+  auto count = [&](int64_t t) {
+    return t < slab.begin ? 0 : (int)max((int64_t)0, min((int64_t)S, slab.end - t));
   };
   auto load_back = [&](int64_t t0, int n) {
     const char *r0 = at_step<T>(a.rec, at.b, a.rb, t0, a.rt, at.d);
@@ -468,7 +575,8 @@ __global__ void __launch_bounds__(256, 2)
       if (s < n) {
         rr[s] = load_step<T, V>(r0);
         rg[s] = load_step<T, V>(g0);
-        r0 += a.rt, g0 += a.gt;
+        advance(r0, a.rt, a.one);
+        advance(g0, a.gt, a.one);
       }
     }
   };
@@ -480,7 +588,8 @@ __global__ void __launch_bounds__(256, 2)
       if (s < n) {
         ri[s] = load_step<T, V>(i0);
         rx[s] = load_step<T, V>(x0);
-        i0 += a.it, x0 += a.xt;
+        advance(i0, a.it, a.one);
+        advance(x0, a.xt, a.one);
       }
     }
     if (n) {
@@ -494,107 +603,44 @@ __global__ void __launch_bounds__(256, 2)
   };
 #pragma unroll
   for (int s = 0; s < S; ++s) rr[s] = ri[s] = rx[s] = rg[s] = Raw<T, V>{};
-#pragma unroll
-  for (int v = 0; v < V; ++v) h[v] = 0.0f;
-  int64_t t0 = ((a.tiles - 1 - rank) * W + wt) * S;
-  int n = steps(t0);
+  int64_t t0 = slab.begin + (slab.end - slab.begin - 1) / S * S;
+  int n = count(t0);
   load_back(t0, n);
   load_fwd(t0, n);
-  uint32_t z = reset_bits(a, at.b, t0, n, at.one_row);
-  float rate[V], gam[V], dl[V];
+  uint32_t marks = load_marks(a, at.b, t0, n, at.one_row);
+  Vec<V> rate, gam, dl = all<V>(0.0f);
 #pragma unroll
-  for (int v = 0; v < V; ++v) {
+  for (int v = 0; v < V; ++v)
     gam[v] = a.dh_last ? a.dh_last[at.b * a.D + at.d + v] : 0.0f;
-    dl[v] = 0.0f;
-  }
+  enter_slab<true>(a, slab, at, gam);
   const bool big = load_rates<V>(a, at, rate);
-  if (TILED && ranks > 1) cluster_barrier();
 
-  int par = 0;
-  for (int64_t k0 = a.tiles - 1; k0 >= 0; k0 -= ranks, par ^= 1) {
+  while (n > 0) {
+    const uint32_t z = mark_bits(a, marks, at.one_row);
     const bool slow = big || n < S || __any_sync(0xffffffffu, z != 0);
     const int64_t t_now = t0;
     const int n_now = n;
-    const uint32_t z_now = z;
-    float E[S][V], SR[S][V], g[S][V];
-    float P[V], in[V];
+    t0 -= S;
+    n = count(t0);
+    marks = load_marks(a, at.b, t0, n, at.one_row);
+    Vec<V> E[S], SR[S], g[S];
     auto back = [&](auto tag) {
       constexpr bool SLOW = decltype(tag)::value;
 #pragma unroll
-      for (int v = 0; v < V; ++v) P[v] = 1.0f, in[v] = 0.0f;
-#pragma unroll
       for (int s = S - 1; s >= 0; --s) {
-        float r[V];
-        unpack<T, V>(rr[s], r);
-        unpack<T, V>(rg[s], g[s]);
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-          const bool reset = SLOW && (z_now >> s & 1);
-          const Decay q = decay<SLOW>(r[v], rate[v], reset);
-          E[s][v] = q.e;
-          SR[s][v] = q.sr;
-          if (SLOW && s >= n_now) E[s][v] = 0.0f, g[s][v] = 0.0f;
-          if (TILED) {
-            const float A = 1.0f - E[s][v];
-            P[v] = reset ? -0.0f : P[v] * A;
-            in[v] = reset ? 0.0f : A * (in[v] + g[s][v]);
-          }
+        const bool reset = SLOW && (z >> s & 1);
+        const Decay<V> q = decay<SLOW>(values<T, V>(rr[s]), rate, reset);
+        E[s] = q.e, SR[s] = q.sr;
+        g[s] = add(gam, values<T, V>(rg[s]));
+        if (!SLOW || s < n_now) {
+          gam = mul(q.a, g[s]);
+          if (reset) gam = all<V>(0.0f);
         }
       }
     };
     if (slow) back(std::true_type{});
     else back(std::false_type{});
-    t0 -= (int64_t)ranks * W * S;
-    n = steps(t0);
     load_back(t0, n);
-
-    if (TILED) {
-#pragma unroll
-      for (int v = 0; v < V; ++v)
-        agg[slot + wt][v * 32 + lane] =
-            make_float2(slow && z_now ? -0.0f : P[v], in[v]);
-      __syncthreads();
-      if (ranks > 1) {
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-          if (v % W != wt) continue;
-          const int c = v * 32 + lane;
-          float2 f = agg[slot + W - 1][c];
-          for (int w = W - 2; w >= 0; --w) {
-            const float2 q = agg[slot + w][c];
-            f.y = through(q.x, q.y, f.y);
-            f.x = __float_as_int(q.x) < 0 ? q.x : q.x * f.x;
-          }
-          for (uint32_t r = 0; r < ranks; ++r) store_pair_at(&cagg[par][rank][c], r, f);
-        }
-        cluster_barrier();
-      }
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        if (v % W != wt) continue;
-        const int c = v * 32 + lane;
-        float y = gam[v];
-        if (ranks > 1) {
-          for (uint32_t r = 0; r < ranks; ++r) {
-            if (r == rank) y = gam[v];
-            const float2 f = cagg[par][r][c];
-            gam[v] = through(f.x, f.y, gam[v]);
-          }
-        }
-        for (int w = W - 1; w >= 0; --w) {
-          pre[slot + w][c] = y;
-          const float2 f = agg[slot + w][c];
-          y = through(f.x, f.y, y);
-        }
-        if (ranks == 1) gam[v] = y;
-      }
-      __syncthreads();
-#pragma unroll
-      for (int v = 0; v < V; ++v) in[v] = pre[slot + wt][v * 32 + lane];
-    } else {
-#pragma unroll
-      for (int v = 0; v < V; ++v) in[v] = gam[v];
-    }
 
     const char *dx0 = at_step<T>(a.dx, at.b, a.dxb, t_now, a.dxt, at.d);
     const char *dr0 = at_step<T>(a.drec, at.b, a.drb, t_now, a.drt, at.d);
@@ -602,74 +648,96 @@ __global__ void __launch_bounds__(256, 2)
     auto finish = [&](auto tag) {
       constexpr bool SLOW = decltype(tag)::value;
 #pragma unroll
-      for (int s = S - 1; s >= 0; --s) {
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-          g[s][v] += in[v];
-          in[v] = SLOW && (z_now >> s & 1) ? 0.0f : (1.0f - E[s][v]) * g[s][v];
-        }
-      }
-      if (!TILED) {
-#pragma unroll
-        for (int v = 0; v < V; ++v) gam[v] = in[v];
-      }
-#pragma unroll
       for (int s = 0; s < S; ++s) {
         if (SLOW && s >= n_now) break;
-        float i[V], x[V], ox[V], orec[V], oinp[V];
-        unpack<T, V>(ri[s], i);
-        unpack<T, V>(rx[s], x);
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-          const bool reset = SLOW && (z_now >> s & 1);
-          const float A = 1.0f - E[s][v];
-          const Feed f = feed(i[v], E[s][v]);
-          const float b = f.ms * x[v];
-          ox[v] = g[s][v] * f.ms;
-          const float gx = ox[v] * x[v];
-          // 1 - sigmoid(inp) = (q - 1) / q and 1 / q = m s_i / m = ms w q
-          const float wq = f.w * f.q;
-          oinp[v] = gx * (1.0f - f.ms * wq);
-          // g (h a - s_i x a^2 / m) = a (g h - g m s_i x a / s), 1 / s = (w q)^2
-          const float q =
-              reset ? 0.0f : A * fmaf(g[s][v], h[v], -(gx * A) * (wq * wq));
-          const float sq = SR[s][v] * q;
-          orec[v] = rate[v] * (SR[s][v] - 1.0f) * sq;
-          dl[v] += sq;
-          h[v] = reset ? b : fmaf(A, h[v], b);
-        }
-        if (at.live) {
-          store_step<T, V>(dx0, ox);
-          store_step<T, V>(dr0, orec);
-          store_step<T, V>(di0, oinp);
-        }
-        dx0 += a.dxt, dr0 += a.drt, di0 += a.dit;
+        const Vec<V> i = values<T, V>(ri[s]), x = values<T, V>(rx[s]);
+        const bool reset = SLOW && (z >> s & 1);
+        const Vec<V> A = fma(E[s], -1.0f, 1.0f);
+        const Feed<V> f = feed<true>(i, E[s], A);
+        const Vec<V> dx = mul(g[s], f.ms), gx = mul(dx, x);
+        // s_i = 1 / q = ms (w q), so dinp = gx (1 - s_i); 1 / s = (w q)^2
+        const Vec<V> wq = mul(f.w, f.q);
+        const Vec<V> gms = mul(gx, mul(f.ms, wq));
+        const Vec<V> dinp = fma(gms, -1.0f, gx);
+        // q = g (h a - s_i x a^2 / m) = a (g h - g m s_i x a / s)
+        Vec<V> q = mul(mul(gx, A), mul(wq, wq));
+        q = mul(A, fma(q, -1.0f, mul(g[s], h)));
+        if (reset) q = all<V>(0.0f);
+        const Vec<V> sq = mul(SR[s], q);
+        const Vec<V> drec = mul(mul(rate, add(SR[s], -1.0f)), sq);
+        dl = add(dl, sq);
+        const Vec<V> b = mul(f.ms, x);
+        if (reset) h = b;
+        else h = fma(A, h, b);
+        store_step<T, V>(dx0, dx);
+        store_step<T, V>(dr0, drec);
+        store_step<T, V>(di0, dinp);
+        advance(dx0, a.dxt, a.one);
+        advance(dr0, a.drt, a.one);
+        advance(di0, a.dit, a.one);
       }
     };
     if (slow) finish(std::true_type{});
     else finish(std::false_type{});
     load_fwd(t0, n);
-    z = reset_bits(a, at.b, t0, n, at.one_row);
   }
-  // the block's sum for dlam
-  if (TILED) {
-    __syncthreads();
-#pragma unroll
-    for (int v = 0; v < V; ++v) pre[slot + wt][v * 32 + lane] = dl[v];
-    __syncthreads();
-  }
-  if (at.live) {
+  if (at.live && slab.index < a.slabs) {
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      if (v % W != wt) continue;
-      float s = dl[v];
-      if (TILED) {
-        const int c = v * 32 + lane;
-        s = pre[slot][c];
-        for (int w = 1; w < W; ++w) s += pre[slot + w][c];
+      a.part[((int64_t)slab.index * a.B + at.b) * a.D + at.d + v] = dl[v];
+      if (a.dh0 && slab.index == 0) a.dh0[at.b * a.D + at.d + v] = gam[v];
+    }
+  }
+}
+
+// One step for many rows (a rollout's): a thread keeps its V channels' rates and
+// takes every gridDim.y-th block of rows.
+template <typename T, int V>
+__global__ void __launch_bounds__(256) scan_step_kernel(const __grid_constant__ ScanArgs a,
+                                                        int cols) {
+  const int64_t unit = (int64_t)blockIdx.x * cols + threadIdx.x % cols, per = a.D / V;
+  const int64_t d = unit * V;
+  const int rows = 256 / cols;
+  if (unit >= per || (int)threadIdx.x >= rows * cols) return;
+  Vec<V> rate;
+  bool big = false;
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    rate[v] = a.c * softplus(a.lam[d + v]);
+    big |= rate[v] > kSeriesMax;
+  }
+  constexpr int R = 4;
+  const int64_t pace = (int64_t)gridDim.y * rows;
+  for (int64_t b0 = (int64_t)blockIdx.y * rows + threadIdx.x / cols; b0 < a.B; b0 += R * pace) {
+    Raw<T, V> rr[R], ri[R], rx[R];
+    Vec<V> h[R];
+    uint8_t z[R];
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const int64_t b = b0 + i * pace;
+      if (b < a.B) {
+        rr[i] = load_step<T, V>(at_step<T>(a.rec, b, a.rb, 0, 0, d));
+        ri[i] = load_step<T, V>(at_step<T>(a.inp, b, a.ib, 0, 0, d));
+        rx[i] = load_step<T, V>(at_step<T>(a.x, b, a.xb, 0, 0, d));
+        z[i] = a.resets ? a.resets[b * a.zb] : 0;
+#pragma unroll
+        for (int v = 0; v < V; ++v) h[i][v] = a.h0 ? a.h0[b * a.D + d + v] : 0.0f;
       }
-      a.part[((int64_t)rank * a.B + at.b) * a.D + at.d + v] = s;
-      if (a.dh0 && rank == 0) a.dh0[at.b * a.D + at.d + v] = gam[v];
+    }
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const int64_t b = b0 + i * pace;
+      if (b >= a.B) break;
+      const Vec<V> r = values<T, V>(rr[i]);
+      const Decay<V> g = big || z[i] ? decay<true>(r, rate, z[i] != 0) : decay<false>(r, rate, false);
+      const Vec<V> f =
+          mul(feed<false>(values<T, V>(ri[i]), g.e, g.a).ms, values<T, V>(rx[i]));
+      const Vec<V> y = z[i] ? f : fma(g.a, h[i], f);
+      store_step<T, V>(at_step<T>(a.h, b, a.hb, 0, 0, d), y);
+      if (a.h_last) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) a.h_last[b * a.D + d + v] = y[v];
+      }
     }
   }
 }
@@ -709,41 +777,37 @@ __global__ void __launch_bounds__(1024) scan_dlam_kernel(const float *part, cons
   if (wy == 0 && rank == 0 && d < D) dlam[d] = -c * s / (1.0f + expf(-lam[d]));
 }
 
-// How a call is laid out.  Rows in one piece where their channels fill the
-// SMs (or there is one stretch); else tiles: ceil(T / 8) warps cover a row of up
-// to 64 steps, and a block has as many groups of lanes as fit; longer rows go
-// by 64-step tiles, and where there are too few rows and channels for the SMs,
-// clusters of up to 16 blocks share a row's tiles.
+// How a call is laid out.  A thread takes a row's channels through all steps
+// where rows and channels fill the SMs (kFull warps) or the row is short; else
+// the row is cut into slabs, whose effect on the state is folded in a first
+// pass.
+constexpr int64_t kFull = 148 * 16;
 struct ScanPlan {
-  bool rows;
-  int V, S, W, Z, ranks;
-  int64_t units, tiles, blocks;
+  int V, slabs, slab_blocks;
+  int64_t units, slab_steps, blocks;
 };
 
 ScanPlan plan_scan(int64_t B, int64_t T, int64_t D, int V) {
   ScanPlan p{};
   p.V = V;
-  p.S = T <= 1 ? 1 : kSteps;
   p.units = B * (D / V);
-  const int64_t groups = (p.units + 31) / 32;
-  p.ranks = 1;
-  p.rows = T <= kSteps || groups >= ROWS_GROUPS;
-  if (p.rows) {
-    p.W = 1;
-    p.tiles = (T + p.S - 1) / p.S;
-    p.Z = kWarps;
-    p.blocks = (groups + p.Z - 1) / p.Z;
-    return p;
+  const int64_t groups = std::max<int64_t>(1, (p.units + 31) / 32);
+  p.slabs = p.slab_blocks = 1;
+  p.slab_steps = T;
+  p.blocks = (groups + kWarps - 1) / kWarps;
+  if (groups < kFull && T >= SLAB_T) {
+    const int64_t want = std::min<int64_t>((SLAB_WARPS + groups - 1) / groups, T / kMinSlab);
+    p.slab_steps = ((T + want - 1) / want + kSteps - 1) / kSteps * kSteps;
+    p.slabs = (int)((T + p.slab_steps - 1) / p.slab_steps);
+    p.slab_blocks = (p.slabs + kWarps - 1) / kWarps;
+    p.blocks = groups;
   }
-  p.W = (int)std::min<int64_t>(kWarps, (T + kSteps - 1) / kSteps);
-  p.Z = (int)std::max<int64_t>(1, std::min<int64_t>(kWarps / p.W, groups));
-  p.tiles = (T + p.W * kSteps - 1) / (p.W * kSteps);
-  const int64_t base = (groups + p.Z - 1) / p.Z;
-  if (p.Z == 1)
-    while (p.ranks < kMaxCluster && base * p.ranks < 2 * 148 && p.tiles >= 2 * p.ranks)
-      p.ranks *= 2;
-  p.blocks = base * p.ranks;
   return p;
+}
+
+// Pairs of the first pass: per block of slabs and per slab (whole blocks).
+int64_t fold_pairs(const ScanPlan &p, int64_t B, int64_t D) {
+  return p.slabs > 1 ? (int64_t)p.slab_blocks * (1 + kWarps) * B * D : 0;
 }
 
 template <typename K, typename... A>
@@ -797,12 +861,9 @@ bool place_tensors(ScanTensor *ts, int n, const int64_t *strides, int64_t T, int
 
 template <typename F>
 void with_plan(int32_t dtype, const ScanPlan &p, F &&f) {
-  using std::integral_constant;
   with_dtype(dtype, [&](auto t) {
-    if (p.V == 2 && p.S == 1) f(t, integral_constant<int, 2>{}, integral_constant<int, 1>{});
-    else if (p.V == 2) f(t, integral_constant<int, 2>{}, integral_constant<int, kSteps>{});
-    else if (p.S == 1) f(t, integral_constant<int, 1>{}, integral_constant<int, 1>{});
-    else f(t, integral_constant<int, 1>{}, integral_constant<int, kSteps>{});
+    if (p.V == 2) f(t, std::integral_constant<int, 2>{});
+    else f(t, std::integral_constant<int, 1>{});
   });
 }
 
@@ -810,6 +871,13 @@ zrl_status scan_launched(const char *what, cudaError_t e) {
   if (e == cudaSuccess) return seq_launched(what);
   (void)cudaGetLastError();  // reported here
   return seq_fail(ZRL_CUDA_ERROR, "%s: %s", what, cudaGetErrorString(e));
+}
+
+void use_plan(ScanArgs &a, const ScanPlan &p, void *workspace) {
+  a.units = p.units;
+  a.slabs = p.slabs;
+  a.slab_steps = p.slab_steps;
+  a.fold = static_cast<float2 *>(workspace);
 }
 
 zrl_status check_scan(const char *what, int64_t B, int64_t T, int64_t D, int32_t dtype, float c) {
@@ -833,6 +901,7 @@ void scan_inputs(ScanArgs &a, const void *x, const void *rec, const void *inp, c
   a.D = D;
   a.K = chunk_starts(T);
   a.c = c;
+  a.one = 1;
   a.zb = strides ? strides[6] : T;
   a.zt = strides ? strides[7] : 1;
 }
@@ -846,11 +915,19 @@ extern "C" int64_t zrl_gated_scan_carry(int64_t B, int64_t T, int64_t D) {
   return B > 0 && D > 0 ? B * chunk_starts(T) * D : 0;
 }
 
+extern "C" int64_t zrl_gated_scan_workspace(int64_t B, int64_t T, int64_t D) {
+  if (B <= 0 || D <= 0) return 0;
+  const int64_t pairs = std::max(fold_pairs(plan_scan(B, T, D, 1), B, D),
+                                 fold_pairs(plan_scan(B, T, D, 2), B, D));
+  return pairs * (int64_t)sizeof(float2);
+}
+
 extern "C" zrl_status zrl_gated_scan(const void *x, const void *rec, const void *inp,
                                      const float *lam, const float *h0, const uint8_t *resets,
                                      int64_t B, int64_t T, int64_t D, int32_t dtype, float c,
                                      const int64_t *strides, void *h, float *h_last,
-                                     float *carry, void *stream) {
+                                     float *carry, void *workspace, int64_t workspace_bytes,
+                                     void *stream) {
   const zrl_status s = check_scan("gated_scan", B, T, D, dtype, c);
   if (s != ZRL_OK) return s;
   if (B == 0 || D == 0) return ZRL_OK;
@@ -872,29 +949,36 @@ extern "C" zrl_status zrl_gated_scan(const void *x, const void *rec, const void 
     return seq_fail(ZRL_NOT_SUPPORTED, "gated_scan: a time stride of 2 GiB or more");
   const ScanPlan p = plan_scan(B, T, D, pairs ? 2 : 1);
   if (p.blocks > 0x7fffffff) return seq_fail(ZRL_NOT_SUPPORTED, "gated_scan: B * D too large");
-  a.units = p.units;
-  a.tiles = p.tiles;
-  cudaError_t e = cudaSuccess;
-  with_plan(dtype, p, [&](auto t, auto v, auto s) {
+  if (workspace_bytes < zrl_gated_scan_workspace(B, T, D) || !aligned(workspace, 16) ||
+      (!workspace && p.slabs > 1))
+    return seq_fail(ZRL_INVALID_ARG, "gated_scan: workspace too small or not aligned");
+  use_plan(a, p, workspace);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  with_plan(dtype, p, [&](auto t, auto v) {
     using E = decltype(t);
-    constexpr int V = decltype(v)::value, S = decltype(s)::value;
-    const dim3 threads(32, p.W, p.Z);
-    cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (p.rows) {
-      scan_rows_kernel<E, V, S><<<(unsigned)p.blocks, threads, 0, st>>>(a);
-      e = cudaGetLastError();
-    } else if constexpr (S == kSteps) {
-      e = launch_cluster(scan_tile_kernel<E, V, S>, (unsigned)p.blocks, threads, p.ranks, st, a);
+    constexpr int V = decltype(v)::value;
+    const dim3 grid((unsigned)p.blocks, (unsigned)p.slab_blocks), threads(32, kWarps);
+    if (T == 1) {
+      const int64_t per = D / V;
+      const int cols = (int)std::min<int64_t>(256, per);
+      const int64_t across = (per + cols - 1) / cols, rows = 256 / cols;
+      const int64_t down = std::min<int64_t>((B + rows - 1) / rows,
+                                             std::max<int64_t>(1, STEP_BLOCKS / across));
+      scan_step_kernel<E, V>
+          <<<dim3((unsigned)across, (unsigned)down), 256, 0, st>>>(a, cols);
+      return;
     }
+    if (p.slabs > 1) scan_fold_kernel<E, V, false><<<grid, threads, 0, st>>>(a);
+    scan_kernel<E, V><<<grid, threads, 0, st>>>(a);
   });
-  return scan_launched("gated_scan", e);
+  return seq_launched("gated_scan");
 }
 
 extern "C" int64_t zrl_gated_scan_grad_workspace(int64_t B, int64_t T, int64_t D) {
   if (B <= 0 || D <= 0) return 0;
-  // dlam's sums, one per row, channel and block of a cluster
-  const int ranks = std::max(plan_scan(B, T, D, 1).ranks, plan_scan(B, T, D, 2).ranks);
-  return B * D * ranks * (int64_t)sizeof(float);
+  // dlam's sums, one per row, channel and slab, on top of the first pass's pairs
+  const int slabs = std::max(plan_scan(B, T, D, 1).slabs, plan_scan(B, T, D, 2).slabs);
+  return zrl_gated_scan_workspace(B, T, D) + B * D * slabs * (int64_t)sizeof(float);
 }
 
 extern "C" zrl_status zrl_gated_scan_grad(
@@ -928,7 +1012,6 @@ extern "C" zrl_status zrl_gated_scan_grad(
   a.drec = drec;
   a.dinp = dinp;
   a.dh0 = dh0;
-  a.part = static_cast<float *>(workspace);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   ScanTensor ts[] = {{x, 0, &a.xb, &a.xt},     {rec, 2, &a.rb, &a.rt},    {inp, 4, &a.ib, &a.it},
                      {dh, 8, &a.gb, &a.gt},    {dx, 10, &a.dxb, &a.dxt},  {drec, 12, &a.drb, &a.drt},
@@ -939,27 +1022,21 @@ extern "C" zrl_status zrl_gated_scan_grad(
   const ScanPlan p = plan_scan(B, T, D, pairs ? 2 : 1);
   if (p.blocks > 0x7fffffff)
     return seq_fail(ZRL_NOT_SUPPORTED, "gated_scan_grad: B * D too large");
-  a.units = p.units;
-  a.tiles = p.tiles;
-  cudaError_t e = cudaSuccess;
+  use_plan(a, p, workspace);
+  a.part = reinterpret_cast<float *>(static_cast<char *>(workspace) +
+                                     zrl_gated_scan_workspace(B, T, D));
   if (B)
-    with_plan(dtype, p, [&](auto t, auto v, auto s) {
+    with_plan(dtype, p, [&](auto t, auto v) {
       using E = decltype(t);
-      constexpr int V = decltype(v)::value, S = decltype(s)::value;
-      const dim3 threads(32, p.W, p.Z);
-      if (p.rows) {
-        scan_grad_kernel<E, V, S, false><<<(unsigned)p.blocks, threads, 0, st>>>(a);
-        e = cudaGetLastError();
-      } else if constexpr (S == kSteps) {
-        e = launch_cluster(scan_grad_kernel<E, V, S, true>, (unsigned)p.blocks, threads, p.ranks,
-                           st, a);
-      }
+      constexpr int V = decltype(v)::value;
+      const dim3 grid((unsigned)p.blocks, (unsigned)p.slab_blocks), threads(32, kWarps);
+      if (p.slabs > 1) scan_fold_kernel<E, V, true><<<grid, threads, 0, st>>>(a);
+      scan_grad_kernel<E, V><<<grid, threads, 0, st>>>(a);
     });
-  if (e == cudaSuccess) {
-    const int64_t rows = B * p.ranks;
-    const int ranks = rows >= 1024 ? 8 : 1;
-    e = launch_cluster(scan_dlam_kernel, (unsigned)((D + 31) / 32 * ranks), dim3(1024), ranks, st,
-                       (const float *)a.part, lam, rows, D, c, dlam);
-  }
+  const int64_t rows = B * p.slabs;
+  const int ranks = rows >= 1024 ? 8 : 1;
+  const cudaError_t e =
+      launch_cluster(scan_dlam_kernel, (unsigned)((D + 31) / 32 * ranks), dim3(1024), ranks, st,
+                     (const float *)a.part, lam, rows, D, c, dlam);
   return scan_launched("gated_scan_grad", e);
 }

@@ -128,7 +128,9 @@ _SIGS = {
                                            C.c_int32, _P, _P]),
     "zrl_kernel_launches": (C.c_int64, [_P]),
     "zrl_set_mirror": (C.c_int, [_P, _P, _P, _P, _P, _P, _P]),
-    "zrl_gated_scan": (C.c_int, [_P] * 6 + [C.c_int64] * 3 + [C.c_int32, C.c_float] + [_P] * 5),
+    "zrl_gated_scan": (C.c_int, [_P] * 6 + [C.c_int64] * 3 + [C.c_int32, C.c_float] + [_P] * 5 +
+                       [C.c_int64, _P]),
+    "zrl_gated_scan_workspace": (C.c_int64, [C.c_int64] * 3),
     "zrl_gated_scan_carry": (C.c_int64, [C.c_int64] * 3),
     "zrl_gated_scan_grad": (C.c_int, [_P] * 9 + [C.c_int64] * 3 + [C.c_int32, C.c_float] +
                             [_P] * 7 + [C.c_int64, _P]),

@@ -150,9 +150,12 @@ def gated_scan(x, rec, inp, lam, h0=None, resets=None, c: float = 8.0, save: boo
     if save:
         carry = torch.empty((B, max(T - 1, 0) // 8, D), dtype=torch.float32, device=dev)
     st = _strides((("x", x), ("rec", rec), ("inp", inp), ("out", out)), resets)
-    _call(N.lib().zrl_gated_scan, dev, x.data_ptr(), rec.data_ptr(), inp.data_ptr(), p_lam,
+    lib = N.lib()
+    nw = lib.zrl_gated_scan_workspace(B, T, D)
+    ws = torch.empty(nw, dtype=torch.uint8, device=dev) if nw else None
+    _call(lib.zrl_gated_scan, dev, x.data_ptr(), rec.data_ptr(), inp.data_ptr(), p_lam,
           p_h0, p_z, B, T, D, dt, c, st, out.data_ptr(), last.data_ptr(),
-          carry.data_ptr() if save else None)
+          carry.data_ptr() if save else None, ws.data_ptr() if nw else None, nw)
     return (out, last, carry) if save else (out, last)
 
 
@@ -178,7 +181,7 @@ def gated_step(x, rec, inp, lam, state, resets=None, c: float = 8.0, out=None):
         z = resets.stride(0) if resets is not None else 0
         st = (C.c_int64 * 10)(x.stride(0), 0, rec.stride(0), 0, inp.stride(0), 0, z, 0, D, 0)
     _call(N.lib().zrl_gated_scan, dev, x.data_ptr(), rec.data_ptr(), inp.data_ptr(), p_lam,
-          p_h0, p_z, B, 1, D, dt, c, st, h.data_ptr(), _f32("out", out, (B, D), dev), None)
+          p_h0, p_z, B, 1, D, dt, c, st, h.data_ptr(), _f32("out", out, (B, D), dev), None, None, 0)
     return h, out
 
 
