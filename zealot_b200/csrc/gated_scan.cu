@@ -15,15 +15,6 @@
 
 #include "seq_common.cuh"
 
-#ifndef STEP_BLOCKS
-#define STEP_BLOCKS 148*8
-#endif
-#ifndef SLAB_T
-#define SLAB_T 128
-#endif
-#ifndef SLAB_WARPS
-#define SLAB_WARPS 148*24
-#endif
 namespace zrl {
 namespace {
 
@@ -37,6 +28,12 @@ constexpr int kChunk = kSteps;
 constexpr float kLog2e = 1.44269504f;
 constexpr float kSeriesMax = 0.35f;
 constexpr float kTinySquare = 7.5231638e-37f;  // 2^-120
+
+// Blocks of 256 threads an SM holds, which bounds their registers.  Measured
+// (device us, 2 / 3 / 4 blocks): forward 1024 x 24 x 512 bf16 35 / 34 / 32, 4096 x
+// 24 x 128 f32 41 / 47 / 55 (spills); gradient of the former 49 / 110 / - (spills).
+template <typename T> constexpr int resident() { return sizeof(T) == 2 ? 4 : 2; }
+constexpr int kGradResident = 2;
 
 struct ScanArgs {
   const void *x, *rec, *inp, *dh;
@@ -353,7 +350,7 @@ struct Slab {
 // pair (P, H): every warp folds its slab, then the block writes, per warp, the
 // pair of the block's slabs before (after) it, and the pair of them all.
 template <typename T, int V, bool BACK>
-__global__ void __launch_bounds__(256) scan_fold_kernel(const __grid_constant__ ScanArgs a) {
+__global__ void __launch_bounds__(256, resident<T>()) scan_fold_kernel(const __grid_constant__ ScanArgs a) {
   constexpr int S = kSteps;
   __shared__ float2 agg[kWarps][32 * V];
   const int lane = threadIdx.x, wt = threadIdx.y;
@@ -473,7 +470,7 @@ __device__ __forceinline__ void enter_slab(const ScanArgs &a, const Slab &slab, 
 // A thread takes its V channels through the steps of its slab, with the loads
 // of the eight steps ahead in flight.
 template <typename T, int V>
-__global__ void __launch_bounds__(256) scan_kernel(const __grid_constant__ ScanArgs a) {
+__global__ void __launch_bounds__(256, resident<T>()) scan_kernel(const __grid_constant__ ScanArgs a) {
   constexpr int S = kSteps;
   const Slab slab(a);
   const Place<V> at(a, slab.group * 32 + threadIdx.x);
@@ -556,7 +553,7 @@ __global__ void __launch_bounds__(256) scan_kernel(const __grid_constant__ ScanA
 // made as its step comes by.  So every gate is computed once and only 1 - a,
 // sigmoid(rec) and g of a stretch are held.
 template <typename T, int V>
-__global__ void __launch_bounds__(256, 2)
+__global__ void __launch_bounds__(256, kGradResident)
     scan_grad_kernel(const __grid_constant__ ScanArgs a) {
   constexpr int S = kSteps;
   const Slab slab(a);
@@ -778,16 +775,19 @@ __global__ void __launch_bounds__(1024) scan_dlam_kernel(const float *part, cons
 }
 
 // How a call is laid out.  A thread takes a row's channels through all steps
-// where rows and channels fill the SMs (kFull warps) or the row is short; else
-// the row is cut into slabs, whose effect on the state is folded in a first
-// pass.
-constexpr int64_t kFull = 148 * 16;
+// where rows and channels fill the SMs (kFull groups of lanes) or the row is
+// short; else the row is cut into slabs, whose effect on the state is folded in
+// a first pass: as many blocks of eight slabs as fill one to three waves of the
+// resident blocks best.  Measured (fold + scan, device us): 1 x 65536 x 512 f32 in
+// 1 / 1.5 / 3 waves 152 / 171 / 169.
+constexpr int kSms = 148;
+constexpr int64_t kFull = kSms * 16;
 struct ScanPlan {
   int V, slabs, slab_blocks;
   int64_t units, slab_steps, blocks;
 };
 
-ScanPlan plan_scan(int64_t B, int64_t T, int64_t D, int V) {
+ScanPlan plan_scan(int64_t B, int64_t T, int64_t D, int V, int resident) {
   ScanPlan p{};
   p.V = V;
   p.units = B * (D / V);
@@ -795,8 +795,15 @@ ScanPlan plan_scan(int64_t B, int64_t T, int64_t D, int V) {
   p.slabs = p.slab_blocks = 1;
   p.slab_steps = T;
   p.blocks = (groups + kWarps - 1) / kWarps;
-  if (groups < kFull && T >= SLAB_T) {
-    const int64_t want = std::min<int64_t>((SLAB_WARPS + groups - 1) / groups, T / kMinSlab);
+  if (groups < kFull && T >= 4 * kMinSlab) {
+    int64_t best = 1;
+    double filled = 0.0;
+    for (int waves = 1; waves <= 3; ++waves) {
+      const int64_t room = (int64_t)waves * kSms * resident;
+      const double f = (double)(room / groups * groups) / room;
+      if (f > filled + 0.05) filled = f, best = room / groups;
+    }
+    const int64_t want = std::min<int64_t>(std::max<int64_t>(1, best) * kWarps, T / kMinSlab);
     p.slab_steps = ((T + want - 1) / want + kSteps - 1) / kSteps * kSteps;
     p.slabs = (int)((T + p.slab_steps - 1) / p.slab_steps);
     p.slab_blocks = (p.slabs + kWarps - 1) / kWarps;
@@ -804,6 +811,7 @@ ScanPlan plan_scan(int64_t B, int64_t T, int64_t D, int V) {
   }
   return p;
 }
+int fwd_resident(int es) { return es == 2 ? resident<__half>() : resident<float>(); }
 
 // Pairs of the first pass: per block of slabs and per slab (whole blocks).
 int64_t fold_pairs(const ScanPlan &p, int64_t B, int64_t D) {
@@ -915,10 +923,13 @@ extern "C" int64_t zrl_gated_scan_carry(int64_t B, int64_t T, int64_t D) {
   return B > 0 && D > 0 ? B * chunk_starts(T) * D : 0;
 }
 
+// Enough for every element type and for one or two channels a lane.
 extern "C" int64_t zrl_gated_scan_workspace(int64_t B, int64_t T, int64_t D) {
   if (B <= 0 || D <= 0) return 0;
-  const int64_t pairs = std::max(fold_pairs(plan_scan(B, T, D, 1), B, D),
-                                 fold_pairs(plan_scan(B, T, D, 2), B, D));
+  int64_t pairs = 0;
+  for (int V = 1; V <= 2; ++V)
+    for (int es = 2; es <= 4; es += 2)
+      pairs = std::max(pairs, fold_pairs(plan_scan(B, T, D, V, fwd_resident(es)), B, D));
   return pairs * (int64_t)sizeof(float2);
 }
 
@@ -947,7 +958,7 @@ extern "C" zrl_status zrl_gated_scan(const void *x, const void *rec, const void 
   bool pairs = false;
   if (!place_tensors(ts, 4, strides, T, D, es, &pairs))
     return seq_fail(ZRL_NOT_SUPPORTED, "gated_scan: a time stride of 2 GiB or more");
-  const ScanPlan p = plan_scan(B, T, D, pairs ? 2 : 1);
+  const ScanPlan p = plan_scan(B, T, D, pairs ? 2 : 1, fwd_resident(es));
   if (p.blocks > 0x7fffffff) return seq_fail(ZRL_NOT_SUPPORTED, "gated_scan: B * D too large");
   if (workspace_bytes < zrl_gated_scan_workspace(B, T, D) || !aligned(workspace, 16) ||
       (!workspace && p.slabs > 1))
@@ -963,7 +974,7 @@ extern "C" zrl_status zrl_gated_scan(const void *x, const void *rec, const void 
       const int cols = (int)std::min<int64_t>(256, per);
       const int64_t across = (per + cols - 1) / cols, rows = 256 / cols;
       const int64_t down = std::min<int64_t>((B + rows - 1) / rows,
-                                             std::max<int64_t>(1, STEP_BLOCKS / across));
+                                             std::max<int64_t>(1, kSms * 4 / across));
       scan_step_kernel<E, V>
           <<<dim3((unsigned)across, (unsigned)down), 256, 0, st>>>(a, cols);
       return;
@@ -977,8 +988,13 @@ extern "C" zrl_status zrl_gated_scan(const void *x, const void *rec, const void 
 extern "C" int64_t zrl_gated_scan_grad_workspace(int64_t B, int64_t T, int64_t D) {
   if (B <= 0 || D <= 0) return 0;
   // dlam's sums, one per row, channel and slab, on top of the first pass's pairs
-  const int slabs = std::max(plan_scan(B, T, D, 1).slabs, plan_scan(B, T, D, 2).slabs);
-  return zrl_gated_scan_workspace(B, T, D) + B * D * slabs * (int64_t)sizeof(float);
+  int64_t bytes = 0;
+  for (int V = 1; V <= 2; ++V) {
+    const ScanPlan p = plan_scan(B, T, D, V, kGradResident);
+    bytes = std::max(bytes, fold_pairs(p, B, D) * (int64_t)sizeof(float2) +
+                                B * D * p.slabs * (int64_t)sizeof(float));
+  }
+  return bytes;
 }
 
 extern "C" zrl_status zrl_gated_scan_grad(
@@ -1019,12 +1035,12 @@ extern "C" zrl_status zrl_gated_scan_grad(
   bool pairs = false;
   if (!place_tensors(ts, 7, strides, T, D, es, &pairs))
     return seq_fail(ZRL_NOT_SUPPORTED, "gated_scan_grad: a time stride of 2 GiB or more");
-  const ScanPlan p = plan_scan(B, T, D, pairs ? 2 : 1);
+  const ScanPlan p = plan_scan(B, T, D, pairs ? 2 : 1, kGradResident);
   if (p.blocks > 0x7fffffff)
     return seq_fail(ZRL_NOT_SUPPORTED, "gated_scan_grad: B * D too large");
   use_plan(a, p, workspace);
   a.part = reinterpret_cast<float *>(static_cast<char *>(workspace) +
-                                     zrl_gated_scan_workspace(B, T, D));
+                                     fold_pairs(p, B, D) * sizeof(float2));
   if (B)
     with_plan(dtype, p, [&](auto t, auto v) {
       using E = decltype(t);
