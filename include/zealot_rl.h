@@ -442,7 +442,7 @@ typedef enum {
 /* Group norm with an activation over channels-last x [N, L, C]: per n and
  * group of C / groups neighbouring channels, over the L rows (positions; 1
  * normalizes every row by itself), y = act(gamma (x - mean) rstd + beta),
- * rstd = 1 / sqrt(population variance + eps).  gamma, beta [C] fp32 or NULL
+ * rstd = 1 / sqrt(population variance + eps); C at most 2^23.  gamma, beta [C] fp32 or NULL
  * (1, 0).  mean, rstd [N, groups] or NULL: what the gradient needs.  strides:
  * (n, l) of x and y, four in all.  y may be x (same strides).  workspace:
  * zrl_group_norm_workspace(..., 0) bytes, 16-byte aligned (NULL if 0).  No

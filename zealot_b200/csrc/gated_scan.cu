@@ -13,6 +13,7 @@
 #include <algorithm>
 #include <type_traits>
 
+#include "column_sum.cuh"
 #include "seq_common.cuh"
 
 namespace zrl {
@@ -20,7 +21,6 @@ namespace {
 
 constexpr int kSteps = 8;       // steps of a stretch
 constexpr int kWarps = 8;       // warps of a block at most
-constexpr int kMaxCluster = 16;
 constexpr int kMinSlab = 32;    // steps of a slab at least
 // The forward call keeps the state before every stretch after the first; the
 // gradient recomputes the states inside a stretch from there.
@@ -229,28 +229,6 @@ __device__ __forceinline__ Feed<V> feed(const Vec<V> &inp, const Vec<V> &e, cons
 // included.
 __device__ __forceinline__ float through(float P, float H, float h) {
   return __float_as_int(P) < 0 ? H : fmaf(P, h, H);
-}
-
-__device__ __forceinline__ uint32_t cluster_rank() {
-  uint32_t r;
-  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ uint32_t cluster_size() {
-  uint32_t r;
-  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ void cluster_barrier() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;"
-               ::: "memory");
-}
-// Stores a pair at the same shared-memory place of another block of the cluster.
-__device__ __forceinline__ void store_pair_at(float2 *p, uint32_t rank, float2 v) {
-  uint32_t a = (uint32_t)__cvta_generic_to_shared(p), r;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(rank));
-  asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(r), "f"(v.x), "f"(v.y)
-               : "memory");
 }
 
 // Element (row b, step t, channel d) of a [B, T, D] tensor; the steps of a stretch
@@ -739,40 +717,15 @@ __global__ void __launch_bounds__(256) scan_step_kernel(const __grid_constant__ 
   }
 }
 
-// dlam = -c sigmoid(lam) * (column sums of part [rows, D]): a cluster takes 32
-// columns, its blocks every ranks-th stretch of rows; all sums in a fixed order.
-__global__ void __launch_bounds__(1024) scan_dlam_kernel(const float *part, const float *lam,
-                                                         int64_t rows, int64_t D, float c,
-                                                         float *dlam) {
-  __shared__ float buf[32][33];
-  __shared__ float2 whole[kMaxCluster][32];
-  const uint32_t ranks = cluster_size(), rank = cluster_rank();
-  const int lane = threadIdx.x & 31, wy = threadIdx.x >> 5;
-  const int64_t d = (int64_t)(blockIdx.x / ranks) * 32 + lane;
-  if (ranks > 1) cluster_barrier();
-  float s = 0.0f;
-  if (d < D) {
-#pragma unroll 4
-    for (int64_t r = (int64_t)rank * 32 + wy; r < rows; r += (int64_t)ranks * 32)
-      s += part[r * D + d];
+// dlam from the column sums
+struct DlamOut {
+  const float *lam;
+  float *dlam;
+  float c;
+  __device__ __forceinline__ void operator()(int64_t d, float sum) const {
+    dlam[d] = -c * sum / (1.0f + expf(-lam[d]));
   }
-  buf[wy][lane] = s;
-  __syncthreads();
-  if (wy == 0) {
-    s = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 32; ++i) s += buf[i][lane];
-    if (ranks > 1) store_pair_at(&whole[rank][lane], 0, make_float2(s, 0.0f));
-  }
-  if (ranks > 1) {
-    cluster_barrier();
-    if (wy == 0) {
-      s = 0.0f;
-      for (uint32_t r = 0; r < ranks; ++r) s += whole[r][lane].x;
-    }
-  }
-  if (wy == 0 && rank == 0 && d < D) dlam[d] = -c * s / (1.0f + expf(-lam[d]));
-}
+};
 
 // How a call is laid out.  A thread takes a row's channels through all steps
 // where rows and channels fill the SMs (kFull groups of lanes) or the row is
@@ -818,27 +771,6 @@ int64_t fold_pairs(const ScanPlan &p, int64_t B, int64_t D) {
   return p.slabs > 1 ? (int64_t)p.slab_blocks * (1 + kWarps) * B * D : 0;
 }
 
-template <typename K, typename... A>
-cudaError_t launch_cluster(K kernel, unsigned blocks, dim3 threads, int ranks, cudaStream_t st,
-                           A... args) {
-  if (ranks > 8) {
-    const cudaError_t e =
-        cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    if (e != cudaSuccess) return e;
-  }
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(blocks);
-  cfg.blockDim = threads;
-  cfg.stream = st;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = (unsigned)ranks;
-  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, args...);
-}
-
 int64_t chunk_starts(int64_t T) { return T > 0 ? (T - 1) / kChunk : 0; }
 
 // A [B, T, D] tensor of a call: where its strides stand in the caller's array
@@ -873,12 +805,6 @@ void with_plan(int32_t dtype, const ScanPlan &p, F &&f) {
     if (p.V == 2) f(t, std::integral_constant<int, 2>{});
     else f(t, std::integral_constant<int, 1>{});
   });
-}
-
-zrl_status scan_launched(const char *what, cudaError_t e) {
-  if (e == cudaSuccess) return seq_launched(what);
-  (void)cudaGetLastError();  // reported here
-  return seq_fail(ZRL_CUDA_ERROR, "%s: %s", what, cudaGetErrorString(e));
 }
 
 void use_plan(ScanArgs &a, const ScanPlan &p, void *workspace) {
@@ -1049,10 +975,6 @@ extern "C" zrl_status zrl_gated_scan_grad(
       if (p.slabs > 1) scan_fold_kernel<E, V, true><<<grid, threads, 0, st>>>(a);
       scan_grad_kernel<E, V><<<grid, threads, 0, st>>>(a);
     });
-  const int64_t rows = B * p.slabs;
-  const int ranks = rows >= 1024 ? 8 : 1;
-  const cudaError_t e =
-      launch_cluster(scan_dlam_kernel, (unsigned)((D + 31) / 32 * ranks), dim3(1024), ranks, st,
-                     (const float *)a.part, lam, rows, D, c, dlam);
-  return scan_launched("gated_scan_grad", e);
+  launch_column_sum(a.part, B * p.slabs, D, DlamOut{lam, dlam, c}, st);
+  return seq_launched("gated_scan_grad");
 }
