@@ -69,8 +69,13 @@ template <typename Out>
 inline void launch_column_sum(const float *part, int64_t rows, int64_t cols, Out out,
                               cudaStream_t st) {
   const int ranks = rows >= 256 ? 8 : 1;
+  const unsigned blocks = (unsigned)((cols + 31) / 32 * ranks);
+  if (ranks == 1) {
+    column_sum_kernel<<<blocks, 1024, 0, st>>>(part, rows, cols, out);
+    return;
+  }
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)((cols + 31) / 32 * ranks));
+  cfg.gridDim = dim3(blocks);
   cfg.blockDim = dim3(1024);
   cfg.stream = st;
   cudaLaunchAttribute at[1];

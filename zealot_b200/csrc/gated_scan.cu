@@ -25,7 +25,6 @@ constexpr int kMinSlab = 32;    // steps of a slab at least
 // The forward call keeps the state before every stretch after the first; the
 // gradient recomputes the states inside a stretch from there.
 constexpr int kChunk = kSteps;
-constexpr float kLog2e = 1.44269504f;
 constexpr float kSeriesMax = 0.35f;
 constexpr float kTinySquare = 7.5231638e-37f;  // 2^-120
 
@@ -52,21 +51,6 @@ struct ScanArgs {
   int32_t one;  // 1
 };
 
-__device__ __forceinline__ float ex2(float v) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
-  return r;
-}
-__device__ __forceinline__ float rcp(float v) {
-  float r;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
-  return r;
-}
-__device__ __forceinline__ float rsq(float v) {
-  float r;
-  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
-  return r;
-}
 // NaN stays NaN, unlike fminf
 __device__ __forceinline__ float min_nan(float a, float b) {
   float r;
@@ -89,79 +73,6 @@ __device__ __forceinline__ float softplus(float v) {
   p = fmaf(z2, p, 1.0f / 3.0f);
   p = fmaf(z2, p, 1.0f);
   return (v > 0.0f ? v : v != v ? v : 0.0f) + 2.0f * z * p;
-}
-
-// V channels' values.  Pairs go through the packed fp32 instructions, which
-// halve the issue slots of everything but the special functions.
-template <int V>
-struct Vec {
-  float v[V];
-  __device__ __forceinline__ float &operator[](int i) { return v[i]; }
-  __device__ __forceinline__ const float &operator[](int i) const { return v[i]; }
-};
-template <int V>
-__device__ __forceinline__ Vec<V> all(float c) {
-  Vec<V> r;
-#pragma unroll
-  for (int i = 0; i < V; ++i) r[i] = c;
-  return r;
-}
-template <int V>
-__device__ __forceinline__ Vec<V> fma(const Vec<V> &a, const Vec<V> &b, const Vec<V> &c) {
-  Vec<V> r;
-  if constexpr (V == 2) {
-    const float2 f = __ffma2_rn(make_float2(a[0], a[1]), make_float2(b[0], b[1]),
-                                make_float2(c[0], c[1]));
-    r[0] = f.x, r[1] = f.y;
-  } else {
-#pragma unroll
-    for (int i = 0; i < V; ++i) r[i] = fmaf(a[i], b[i], c[i]);
-  }
-  return r;
-}
-template <int V>
-__device__ __forceinline__ Vec<V> mul(const Vec<V> &a, const Vec<V> &b) {
-  Vec<V> r;
-  if constexpr (V == 2) {
-    const float2 f = __fmul2_rn(make_float2(a[0], a[1]), make_float2(b[0], b[1]));
-    r[0] = f.x, r[1] = f.y;
-  } else {
-#pragma unroll
-    for (int i = 0; i < V; ++i) r[i] = a[i] * b[i];
-  }
-  return r;
-}
-template <int V>
-__device__ __forceinline__ Vec<V> add(const Vec<V> &a, const Vec<V> &b) {
-  Vec<V> r;
-  if constexpr (V == 2) {
-    const float2 f = __fadd2_rn(make_float2(a[0], a[1]), make_float2(b[0], b[1]));
-    r[0] = f.x, r[1] = f.y;
-  } else {
-#pragma unroll
-    for (int i = 0; i < V; ++i) r[i] = a[i] + b[i];
-  }
-  return r;
-}
-template <int V>
-__device__ __forceinline__ Vec<V> fma(const Vec<V> &a, float b, const Vec<V> &c) {
-  return fma(a, all<V>(b), c);
-}
-template <int V>
-__device__ __forceinline__ Vec<V> fma(const Vec<V> &a, const Vec<V> &b, float c) {
-  return fma(a, b, all<V>(c));
-}
-template <int V>
-__device__ __forceinline__ Vec<V> fma(const Vec<V> &a, float b, float c) {
-  return fma(a, all<V>(b), all<V>(c));
-}
-template <int V>
-__device__ __forceinline__ Vec<V> mul(const Vec<V> &a, float b) {
-  return mul(a, all<V>(b));
-}
-template <int V>
-__device__ __forceinline__ Vec<V> add(const Vec<V> &a, float b) {
-  return add(a, all<V>(b));
 }
 
 // The gates of one step.  With u = rate sigmoid(rec), e = 1 - a = 1 - exp(-u)
@@ -237,12 +148,6 @@ template <typename T>
 __device__ __forceinline__ const char *at_step(const void *p, int64_t b, int64_t sb, int64_t t,
                                                int32_t st, int64_t d) {
   return static_cast<const char *>(p) + (b * sb + d) * (int64_t)sizeof(T) + t * st;
-}
-template <typename T, int V>
-__device__ __forceinline__ Vec<V> values(const Raw<T, V> &raw) {
-  Vec<V> r;
-  unpack<T, V>(raw, r.v);
-  return r;
 }
 template <typename T, int V>
 __device__ __forceinline__ Raw<T, V> load_step(const char *p) {

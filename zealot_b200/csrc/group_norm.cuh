@@ -1,0 +1,136 @@
+// group_norm.cuh -- what the forms of group norm share: arguments, activations,
+// parameters.
+#pragma once
+
+#include "seq_common.cuh"
+
+namespace zrl {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kSms = 148;
+
+struct NormArgs {
+  const void *x, *dy;
+  const float *gamma, *beta;
+  void *y, *dx;
+  float *mean, *rstd, *part;
+  float2 *means;
+  int64_t N, L, sxn, sxl, syn, syl, sdn, sdl;  // strides of x, y / dy, dx
+  int32_t C, G, w, act;
+  float eps;
+  bool wide;    // gamma and beta start on 16 bytes
+  int32_t one;  // 1
+  // lanes and tiles: lanes per group; groups of a block, rows of a block or tile
+  int32_t p, gb, rb;
+  // samples: channels of a block at most, parts of a wide group, stretches of
+  // positions, positions of one
+  int32_t cols, parts, stretches;
+  int64_t stretch;
+};
+
+// Phi(z), the normal distribution's, within 1e-7, and exp(-z^2 / 2): formula
+// 7.1.26 of Abramowitz and Stegun's Handbook (Hastings), erfc(u) = (a1 t + ... +
+// a5 t^5) exp(-u^2) with t = 1 / (1 + p u), at u = |z| / sqrt 2.
+template <int V>
+__device__ __forceinline__ Vec<V> normal_cdf(const Vec<V> &z, Vec<V> &e) {
+  Vec<V> u, t;
+  e = mul(mul(z, z), -0.5f * kLog2e);
+#pragma unroll
+  for (int i = 0; i < V; ++i) e[i] = ex2(e[i]), u[i] = fabsf(z[i]);
+  t = fma(u, 0.3275911f * 0.70710678f, 1.0f);
+#pragma unroll
+  for (int i = 0; i < V; ++i) t[i] = rcp(t[i]);
+  Vec<V> p = fma(t, 1.061405429f, -1.453152027f);
+  p = fma(p, t, 1.421413741f);
+  p = fma(p, t, -0.284496736f);
+  p = fma(p, t, 0.254829592f);
+  p = mul(mul(p, t), mul(e, 0.5f));  // the tail beyond |z|
+  t = fma(p, -1.0f, 1.0f);
+#pragma unroll
+  for (int i = 0; i < V; ++i) p[i] = z[i] < 0.0f ? p[i] : t[i];
+  return p;
+}
+
+// act(z).  ELU's and SiLU's exponentials are absolute to 1e-7 of 1, as z itself
+// is of max(1, |z|).
+template <int V>
+__device__ __forceinline__ void act_values(Vec<V> &z, int act) {
+  if (act == ZRL_ACT_ELU) {
+    const Vec<V> t = mul(z, kLog2e);
+#pragma unroll
+    for (int i = 0; i < V; ++i) z[i] = z[i] > 0.0f ? z[i] : ex2(t[i]) - 1.0f;
+  } else if (act == ZRL_ACT_SILU) {
+    Vec<V> t = mul(z, -kLog2e);
+#pragma unroll
+    for (int i = 0; i < V; ++i) t[i] = ex2(t[i]);
+    t = add(t, 1.0f);
+#pragma unroll
+    for (int i = 0; i < V; ++i) t[i] = rcp(t[i]);
+    z = mul(z, t);
+  } else if (act == ZRL_ACT_GELU) {
+    Vec<V> e;
+    z = mul(z, normal_cdf(z, e));
+  }
+}
+// z becomes act'(z).
+template <int V>
+__device__ __forceinline__ void act_slopes(Vec<V> &z, int act) {
+  if (act == ZRL_ACT_ELU) {
+    const Vec<V> t = mul(z, kLog2e);
+#pragma unroll
+    for (int i = 0; i < V; ++i) z[i] = z[i] > 0.0f ? 1.0f : ex2(t[i]);
+  } else if (act == ZRL_ACT_SILU) {
+    Vec<V> t = mul(z, -kLog2e);
+#pragma unroll
+    for (int i = 0; i < V; ++i) t[i] = ex2(t[i]);
+    t = add(t, 1.0f);
+#pragma unroll
+    for (int i = 0; i < V; ++i) t[i] = rcp(t[i]);
+    z = fma(mul(z, t), fma(t, -1.0f, 1.0f), t);
+  } else if (act == ZRL_ACT_GELU) {
+    Vec<V> e;
+    const Vec<V> p = normal_cdf(z, e);
+    z = fma(mul(z, 0.39894228f), e, p);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) z[i] = z[i] == z[i] ? 1.0f : z[i];
+  }
+}
+
+// gamma or beta of V channels from p + at, or c where p is NULL; one access of
+// 16 bytes for four where wide says that they are aligned.
+template <int V>
+__device__ __forceinline__ Vec<V> params(const float *p, int64_t at, float c, bool wide) {
+  Vec<V> r = all<V>(c);
+  if (!p) return r;
+  if constexpr (V % 4 == 0) {
+    if (wide) {
+#pragma unroll
+      for (int i = 0; i < V; i += 4) {
+        const float4 f = *reinterpret_cast<const float4 *>(p + at + i);
+        r[i] = f.x, r[i + 1] = f.y, r[i + 2] = f.z, r[i + 3] = f.w;
+      }
+      return r;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < V; ++i) r[i] = p[at + i];
+  return r;
+}
+
+// Each v summed over the p (a power of two) neighbouring lanes of a group.
+template <int U>
+__device__ __forceinline__ void lanes_sum(float (&v)[U], int p) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1)
+    if (p > o) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) v[u] += __shfl_xor_sync(0xffffffffu, v[u], o);
+    }
+}
+
+extern __shared__ __align__(16) unsigned char norm_smem[];
+
+}  // namespace
+}  // namespace zrl

@@ -8,6 +8,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "zrl_internal.h"
 
 namespace zrl {
@@ -92,6 +94,123 @@ __device__ __forceinline__ Raw<T, V> pack(const float *in) {
   return raw;
 }
 
+constexpr float kLog2e = 1.44269504f;
+
+// The special functions' approximate forms: 2^v, 1 / v and 1 / sqrt(v) within a
+// few units in the last place (PTX's stated bounds), subnormals as zero.
+__device__ __forceinline__ float ex2(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float rcp(float v) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float rsq(float v) {
+  float r;
+  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+// V channels' values.  Pairs go through the packed fp32 instructions, which
+// halve the issue slots of everything but the special functions.
+template <int V>
+struct Vec {
+  float v[V];
+  __device__ __forceinline__ float &operator[](int i) { return v[i]; }
+  __device__ __forceinline__ const float &operator[](int i) const { return v[i]; }
+};
+template <int V>
+__device__ __forceinline__ Vec<V> all(float c) {
+  Vec<V> r;
+#pragma unroll
+  for (int i = 0; i < V; ++i) r[i] = c;
+  return r;
+}
+template <int V>
+__device__ __forceinline__ Vec<V> fma(const Vec<V> &a, const Vec<V> &b, const Vec<V> &c) {
+  Vec<V> r;
+  if constexpr (V % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < V; i += 2) {
+      const float2 f = __ffma2_rn(make_float2(a[i], a[i + 1]), make_float2(b[i], b[i + 1]),
+                                  make_float2(c[i], c[i + 1]));
+      r[i] = f.x, r[i + 1] = f.y;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) r[i] = fmaf(a[i], b[i], c[i]);
+  }
+  return r;
+}
+template <int V>
+__device__ __forceinline__ Vec<V> mul(const Vec<V> &a, const Vec<V> &b) {
+  Vec<V> r;
+  if constexpr (V % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < V; i += 2) {
+      const float2 f = __fmul2_rn(make_float2(a[i], a[i + 1]), make_float2(b[i], b[i + 1]));
+      r[i] = f.x, r[i + 1] = f.y;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) r[i] = a[i] * b[i];
+  }
+  return r;
+}
+template <int V>
+__device__ __forceinline__ Vec<V> add(const Vec<V> &a, const Vec<V> &b) {
+  Vec<V> r;
+  if constexpr (V % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < V; i += 2) {
+      const float2 f = __fadd2_rn(make_float2(a[i], a[i + 1]), make_float2(b[i], b[i + 1]));
+      r[i] = f.x, r[i + 1] = f.y;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) r[i] = a[i] + b[i];
+  }
+  return r;
+}
+template <int V>
+__device__ __forceinline__ Vec<V> fma(const Vec<V> &a, float b, const Vec<V> &c) {
+  return fma(a, all<V>(b), c);
+}
+template <int V>
+__device__ __forceinline__ Vec<V> fma(const Vec<V> &a, const Vec<V> &b, float c) {
+  return fma(a, b, all<V>(c));
+}
+template <int V>
+__device__ __forceinline__ Vec<V> fma(const Vec<V> &a, float b, float c) {
+  return fma(a, all<V>(b), all<V>(c));
+}
+template <int V>
+__device__ __forceinline__ Vec<V> mul(const Vec<V> &a, float b) {
+  return mul(a, all<V>(b));
+}
+template <int V>
+__device__ __forceinline__ Vec<V> add(const Vec<V> &a, float b) {
+  return add(a, all<V>(b));
+}
+template <int V>
+__device__ __forceinline__ float sum(const Vec<V> &a) {
+  if constexpr (V == 1) {
+    return a[0];
+  } else {
+    Vec<V / 2> h, l;
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) h[i] = a[i], l[i] = a[i + V / 2];
+    return sum(add(h, l));
+  }
+}
+template <typename T, int V>
+__device__ __forceinline__ Vec<V> values(const Raw<T, V> &raw) {
+  Vec<V> r;
+  unpack<T, V>(raw, r.v);
+  return r;
+}
 template <typename T, int V>
 __device__ __forceinline__ void load_vec(const T *p, float *out) {
   const Raw<T, V> raw = *reinterpret_cast<const Raw<T, V> *>(p);

@@ -15,6 +15,7 @@ A refused argument raises ``native.ZrlError`` or ``TypeError``.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 
 import torch
 
@@ -24,6 +25,10 @@ from . import native as N
 ACTIVATIONS = {"none": 0, "elu": 1, "silu": 2, "gelu": 3}
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_F32 = torch.float32
+# the cheap forms of torch.cuda.current_device() and current_stream().cuda_stream
+_device = torch._C._cuda_getDevice
+_stream = torch._C._cuda_getCurrentRawStream
 
 
 def _invalid(msg: str):
@@ -33,27 +38,43 @@ def _invalid(msg: str):
 def _dtype(x) -> int:
     if not x.is_cuda:
         raise TypeError(f"tensor on {x.device}: these operators take CUDA tensors")
-    try:
-        return _DTYPES[x.dtype]
-    except KeyError:
-        raise TypeError(f"element type {x.dtype}: float32, bfloat16 or float16") from None
+    dt = _DTYPES.get(x.dtype)
+    if dt is None:
+        raise TypeError(f"element type {x.dtype}: float32, bfloat16 or float16")
+    return dt
 
 
 def _call(fn, device, *args):
     """fn(*args, stream) on the device's current stream."""
-    if torch.cuda.current_device() == device.index:
-        status = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    i = device.index
+    if _device() == i:
+        status = fn(*args, _stream(i))
     else:
-        with torch.cuda.device(device):
-            status = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+        with torch.cuda.device(i):
+            status = fn(*args, _stream(i))
     if status != N.OK:
         raise N.ZrlError(status, N.lib().zrl_last_error(None).decode())
+
+
+@functools.lru_cache(maxsize=4096)
+def _bytes(name: str, *sizes) -> int:
+    """The workspace of a call of these sizes."""
+    return getattr(N.lib(), name)(*sizes)
+
+
+def _workspace(name: str, f32, *sizes):
+    """(tensor to keep until the call, address, bytes); f32: an fp32 tensor of the device."""
+    n = _bytes(name, *sizes)
+    if not n:
+        return None, None, 0
+    t = f32.new_empty(n // 4)
+    return t, t.data_ptr(), n
 
 
 def _same(name, t, shape, dtype, device):
     if t.dtype != dtype or t.device != device:
         raise TypeError(f"{name}: {t.dtype} on {t.device}, expected {dtype} on {device}")
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise _invalid(f"{name}: shape {tuple(t.shape)}, expected {tuple(shape)}")
 
 
@@ -68,11 +89,19 @@ def _row_stride(name, t, D):
     return v.stride(0)
 
 
+def _dense_like(x):
+    """An empty dense tensor of x's shape, in the order the shape is written."""
+    if x.is_contiguous():
+        return torch.empty_like(x)
+    return torch.empty(x.shape, dtype=x.dtype, device=x.device)
+
+
 def _f32(name, t, shape, device):
     """The address of an fp32 parameter, state or statistic; None stays None."""
     if t is None:
         return None
-    _same(name, t, shape, torch.float32, device)
+    if t.dtype != _F32 or t.device != device or t.shape != shape:
+        _same(name, t, shape, _F32, device)
     if not t.is_contiguous():
         raise _invalid(f"{name}: not contiguous")
     return t.data_ptr()
@@ -87,37 +116,43 @@ def _bt(name, t):
 
 def _like(x):
     """An empty tensor of x's shape: time-major in memory where x is."""
+    if x.is_contiguous():
+        return torch.empty_like(x)
     B, T, D = x.shape
     if x.stride(0) < x.stride(1) and B > 1 and T > 1:
         return torch.empty((T, B, D), dtype=x.dtype, device=x.device).transpose(0, 1)
     return torch.empty((B, T, D), dtype=x.dtype, device=x.device)
 
 
-def _scan_inputs(x, rec, inp, lam, h0, resets, shape):
+def _scan_inputs(x, rec, inp, lam, h0, resets, shape, dev):
     """Checks what forward and gradient share; (lam, h0, resets) addresses."""
-    dev = x.device
     _same("rec", rec, shape, x.dtype, dev)
     _same("inp", inp, shape, x.dtype, dev)
     D = shape[-1]
+    p_z = None
     if resets is not None:
         if resets.dtype not in (torch.uint8, torch.bool) or resets.device != dev:
             raise TypeError("resets: uint8 or bool on x's device")
         if resets.shape != shape[:-1]:
             raise _invalid(f"resets: shape {tuple(resets.shape)}, expected {tuple(shape[:-1])}")
-    return (_f32("lam", lam, (D,), dev), _f32("h0", h0, (shape[0], D), dev),
-            None if resets is None else resets.data_ptr())
+        p_z = resets.data_ptr()
+    return _f32("lam", lam, (D,), dev), _f32("h0", h0, (shape[0], D), dev), p_z
 
 
-def _strides(tensors, resets):
+def _strides(tensors, names, resets):
     """The (batch, time) strides of the call's tensors with resets' in fourth
     place, or None where all are dense in [B, T, D] order."""
-    if all(t.is_contiguous() for _, t in tensors) and (resets is None or resets.is_contiguous()):
-        return None
+    for t in tensors:
+        if not t.is_contiguous():
+            break
+    else:
+        if resets is None or resets.is_contiguous():
+            return None
     st = []
-    for i, (name, t) in enumerate(tensors):
+    for i, t in enumerate(tensors):
         if i == 3:
             st += (0, 0) if resets is None else resets.stride()
-        st += _bt(name, t)
+        st += _bt(names[i], t)
     return (C.c_int64 * len(st))(*st)
 
 
@@ -139,23 +174,19 @@ def gated_scan(x, rec, inp, lam, h0=None, resets=None, c: float = 8.0, save: boo
     if x.dim() != 3:
         raise _invalid(f"x: {x.dim()} axes, expected [B, T, D]")
     dt, dev, shape = _dtype(x), x.device, x.shape
-    p_lam, p_h0, p_z = _scan_inputs(x, rec, inp, lam, h0, resets, shape)
+    p_lam, p_h0, p_z = _scan_inputs(x, rec, inp, lam, h0, resets, shape, dev)
     B, T, D = shape
     if out is None:
         out = _like(x)
     else:
         _same("out", out, shape, x.dtype, dev)
-    last = torch.empty((B, D), dtype=torch.float32, device=dev)
-    carry = None
-    if save:
-        carry = torch.empty((B, max(T - 1, 0) // 8, D), dtype=torch.float32, device=dev)
-    st = _strides((("x", x), ("rec", rec), ("inp", inp), ("out", out)), resets)
-    lib = N.lib()
-    nw = lib.zrl_gated_scan_workspace(B, T, D)
-    ws = torch.empty(nw, dtype=torch.uint8, device=dev) if nw else None
-    _call(lib.zrl_gated_scan, dev, x.data_ptr(), rec.data_ptr(), inp.data_ptr(), p_lam,
+    last = lam.new_empty((B, D)) if h0 is None else torch.empty_like(h0)
+    carry = lam.new_empty((B, max(T - 1, 0) // 8, D)) if save else None
+    ws, p_ws, nw = _workspace("zrl_gated_scan_workspace", lam, B, T, D)
+    st = _strides((x, rec, inp, out), ("x", "rec", "inp", "out"), resets)
+    _call(N.lib().zrl_gated_scan, dev, x.data_ptr(), rec.data_ptr(), inp.data_ptr(), p_lam,
           p_h0, p_z, B, T, D, dt, c, st, out.data_ptr(), last.data_ptr(),
-          carry.data_ptr() if save else None, ws.data_ptr() if nw else None, nw)
+          carry.data_ptr() if save else None, p_ws, nw)
     return (out, last, carry) if save else (out, last)
 
 
@@ -168,11 +199,11 @@ def gated_step(x, rec, inp, lam, state, resets=None, c: float = 8.0, out=None):
     dt, dev, shape = _dtype(x), x.device, x.shape
     if state is None:
         raise _invalid("state: a float32 tensor [B, D]")
-    p_lam, p_h0, p_z = _scan_inputs(x, rec, inp, lam, state, resets, shape)
+    p_lam, p_h0, p_z = _scan_inputs(x, rec, inp, lam, state, resets, shape, dev)
     B, D = shape
-    h = torch.empty((B, D), dtype=x.dtype, device=dev)
+    h = _dense_like(x)
     if out is None:
-        out = torch.empty((B, D), dtype=torch.float32, device=dev)
+        out = torch.empty_like(state)
     st = None
     if not (x.is_contiguous() and rec.is_contiguous() and inp.is_contiguous() and
             (resets is None or resets.is_contiguous())):
@@ -181,7 +212,7 @@ def gated_step(x, rec, inp, lam, state, resets=None, c: float = 8.0, out=None):
         z = resets.stride(0) if resets is not None else 0
         st = (C.c_int64 * 10)(x.stride(0), 0, rec.stride(0), 0, inp.stride(0), 0, z, 0, D, 0)
     _call(N.lib().zrl_gated_scan, dev, x.data_ptr(), rec.data_ptr(), inp.data_ptr(), p_lam,
-          p_h0, p_z, B, 1, D, dt, c, st, h.data_ptr(), _f32("out", out, (B, D), dev), None, None, 0)
+          p_h0, p_z, B, 1, D, dt, c, st, h.data_ptr(), _f32("out", out, shape, dev), None, None, 0)
     return h, out
 
 
@@ -196,7 +227,7 @@ def gated_scan_grad(x, rec, inp, lam, dh, carry, dh_last=None, h0=None, resets=N
     if x.dim() != 3:
         raise _invalid(f"x: {x.dim()} axes, expected [B, T, D]")
     dt, dev, shape = _dtype(x), x.device, x.shape
-    p_lam, p_h0, p_z = _scan_inputs(x, rec, inp, lam, h0, resets, shape)
+    p_lam, p_h0, p_z = _scan_inputs(x, rec, inp, lam, h0, resets, shape, dev)
     B, T, D = shape
     _same("dh", dh, shape, x.dtype, dev)
     p_dl = _f32("dh_last", dh_last, (B, D), dev)
@@ -207,17 +238,15 @@ def gated_scan_grad(x, rec, inp, lam, dh, carry, dh_last=None, h0=None, resets=N
         for name, t in zip(("dx", "drec", "dinp"), out, strict=True):
             _same(name, t, shape, x.dtype, dev)
     dx, drec, dinp = out
-    dlam = torch.empty(D, dtype=torch.float32, device=dev)
-    dh0 = None if h0 is None else torch.empty((B, D), dtype=torch.float32, device=dev)
-    lib = N.lib()
-    nw = lib.zrl_gated_scan_grad_workspace(B, T, D)
-    ws = torch.empty(nw, dtype=torch.uint8, device=dev)
-    st = _strides((("x", x), ("rec", rec), ("inp", inp), ("dh", dh), ("dx", dx), ("drec", drec),
-                   ("dinp", dinp)), resets)
-    _call(lib.zrl_gated_scan_grad, dev, x.data_ptr(), rec.data_ptr(), inp.data_ptr(), p_lam,
+    dlam = torch.empty_like(lam)
+    dh0 = None if h0 is None else torch.empty_like(h0)
+    ws, p_ws, nw = _workspace("zrl_gated_scan_grad_workspace", lam, B, T, D)
+    st = _strides((x, rec, inp, dh, dx, drec, dinp),
+                  ("x", "rec", "inp", "dh", "dx", "drec", "dinp"), resets)
+    _call(N.lib().zrl_gated_scan_grad, dev, x.data_ptr(), rec.data_ptr(), inp.data_ptr(), p_lam,
           p_h0, p_z, p_c, dh.data_ptr(), p_dl, B, T, D, dt, c, st, dx.data_ptr(),
           drec.data_ptr(), dinp.data_ptr(), dlam.data_ptr(),
-          None if dh0 is None else dh0.data_ptr(), ws.data_ptr(), nw)
+          None if dh0 is None else dh0.data_ptr(), p_ws, nw)
     return dx, drec, dinp, dlam, dh0
 
 
@@ -251,10 +280,15 @@ def _norm_shape(x, groups, act):
     return dt, x.shape[0], L, Cn, ACTIVATIONS[act]
 
 
-def _norm_strides(tensors):
-    if all(t.is_contiguous() for _, t in tensors) or not tensors[0][1].numel():
+def _norm_strides(tensors, names):
+    for t in tensors:
+        if not t.is_contiguous():
+            break
+    else:
         return None
-    st = [v for name, t in tensors for v in _nl(name, t)]
+    if not tensors[0].numel():
+        return None
+    st = [v for name, t in zip(names, tensors) for v in _nl(name, t)]
     return (C.c_int64 * len(st))(*st)
 
 
@@ -272,19 +306,26 @@ def group_norm(x, groups: int, gamma=None, beta=None, act: str = "elu", eps: flo
     dev = x.device
     p_g, p_b = _f32("gamma", gamma, (Cn,), dev), _f32("beta", beta, (Cn,), dev)
     if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=dev)
+        out = _dense_like(x)
     else:
         _same("out", out, x.shape, x.dtype, dev)
-    mean = rstd = None
+    f32 = gamma if gamma is not None else x if dt == 0 else None
     if save:
-        mean, rstd = torch.empty((2, n, groups), dtype=torch.float32, device=dev).unbind(0)
-    lib = N.lib()
-    nw = lib.zrl_group_norm_workspace(n, L, Cn, groups, 0)
-    ws = torch.empty(nw, dtype=torch.uint8, device=dev) if nw else None
-    _call(lib.zrl_group_norm, dev, x.data_ptr(), p_g, p_b, n, L, Cn, groups, dt, a, eps,
-          _norm_strides((("x", x), ("out", out))), out.data_ptr(),
-          mean.data_ptr() if save else None, rstd.data_ptr() if save else None,
-          ws.data_ptr() if nw else None, nw)
+        if f32 is None:
+            mean = torch.empty((n, groups), dtype=_F32, device=dev)
+        else:
+            mean = f32.new_empty((n, groups))
+        rstd = torch.empty_like(mean)
+        p_m, p_r = mean.data_ptr(), rstd.data_ptr()
+    else:
+        p_m = p_r = None
+    p_ws, nw = None, 0
+    if x.numel():
+        if f32 is None and _bytes("zrl_group_norm_workspace", n, L, Cn, groups, 0):
+            f32 = mean if save else torch.empty(0, dtype=_F32, device=dev)
+        ws, p_ws, nw = _workspace("zrl_group_norm_workspace", f32, n, L, Cn, groups, 0)
+    _call(N.lib().zrl_group_norm, dev, x.data_ptr(), p_g, p_b, n, L, Cn, groups, dt, a, eps,
+          _norm_strides((x, out), ("x", "out")), out.data_ptr(), p_m, p_r, p_ws, nw)
     return (out, mean, rstd) if save else out
 
 
@@ -297,16 +338,15 @@ def group_norm_grad(x, dy, groups: int, gamma, beta, mean, rstd, act: str = "elu
     p_g, p_b = _f32("gamma", gamma, (Cn,), dev), _f32("beta", beta, (Cn,), dev)
     p_m, p_r = _f32("mean", mean, (n, groups), dev), _f32("rstd", rstd, (n, groups), dev)
     if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=dev)
+        out = _dense_like(x)
     else:
         _same("out", out, x.shape, x.dtype, dev)
-    dgamma, dbeta = torch.empty((2, Cn), dtype=torch.float32, device=dev).unbind(0)
-    lib = N.lib()
-    nw = lib.zrl_group_norm_workspace(n, L, Cn, groups, 1)
-    ws = torch.empty(nw, dtype=torch.uint8, device=dev) if nw else None
-    _call(lib.zrl_group_norm_grad, dev, x.data_ptr(), dy.data_ptr(), p_g, p_b, p_m, p_r, n, L,
-          Cn, groups, dt, a, _norm_strides((("x", x), ("dy", dy), ("out", out))),
-          out.data_ptr(), dgamma.data_ptr(), dbeta.data_ptr(), ws.data_ptr() if nw else None, nw)
+    dgamma = mean.new_empty(Cn) if gamma is None else torch.empty_like(gamma)
+    dbeta = torch.empty_like(dgamma)
+    ws, p_ws, nw = _workspace("zrl_group_norm_workspace", mean, n, L, Cn, groups, 1)
+    _call(N.lib().zrl_group_norm_grad, dev, x.data_ptr(), dy.data_ptr(), p_g, p_b, p_m, p_r, n, L,
+          Cn, groups, dt, a, _norm_strides((x, dy, out), ("x", "dy", "out")), out.data_ptr(),
+          dgamma.data_ptr(), dbeta.data_ptr(), p_ws, nw)
     return out, dgamma, dbeta
 
 
@@ -330,7 +370,7 @@ def dropout(x, p: float, seed: int, stream: int = 0, rows=None, residual=None, o
     if residual is not None:
         _same("residual", residual, x.shape, x.dtype, x.device)
     if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        out = _dense_like(x)
     else:
         _same("out", out, x.shape, x.dtype, x.device)
     n = x.numel() // D if D else 0
@@ -340,10 +380,10 @@ def dropout(x, p: float, seed: int, stream: int = 0, rows=None, residual=None, o
         if D and rows.numel() != n:
             raise _invalid(f"rows: {rows.numel()} numbers for {n} rows")
     strides = None
-    if n:
-        st = [D if t is None or t.is_contiguous() else _row_stride(name, t, D)
-              for name, t in (("x", x), ("residual", residual), ("out", out))]
-        strides = None if st == [D, D, D] else (C.c_int64 * 3)(*st)
+    if n and not (x.is_contiguous() and out.is_contiguous() and
+                  (residual is None or residual.is_contiguous())):
+        strides = (C.c_int64 * 3)(*(D if t is None else _row_stride(name, t, D) for name, t in
+                                    (("x", x), ("residual", residual), ("out", out))))
     _call(N.lib().zrl_dropout, x.device, x.data_ptr(),
           None if residual is None else residual.data_ptr(),
           None if rows is None else rows.data_ptr(), n, D, dt, p, seed, stream, strides,
