@@ -3,6 +3,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <initializer_list>
 #include <type_traits>
 
 #include "philox.cuh"
@@ -16,38 +17,109 @@ struct DropoutArgs {
   const int64_t *rows;
   void *y;
   int64_t sx, sr, sy;  // row strides, elements
-  int64_t N, row0;     // rows, number of the first (rows == NULL)
-  int32_t D, groups;   // columns, groups of 8 columns
+  int64_t N, row0;     // rows of this launch, number of the first (rows == NULL)
+  int32_t D, groups;   // columns; groups of 8 columns, or segments of 256
   uint32_t drop;       // a lane below this is dropped
   float scale;
   uint2 key;
   uint32_t stream_id;
+  uint32_t magic, shift;  // e / groups = umulhi(e, magic) >> shift, for e < 2^31
 };
 
-// One thread per group of eight columns.
-template <typename T>
-__global__ void __launch_bounds__(256) dropout_kernel(const DropoutArgs a) {
-  const int64_t total = a.N * a.groups;
-  for (int64_t e = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; e < total;
-       e += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t row = e / a.groups;
-    const int g = (int)(e - row * a.groups);
-    const int64_t id = a.rows ? a.rows[row] : row;
-    const uint4 w = philox4x32_10(
-        make_uint4((uint32_t)g, (uint32_t)id, (uint32_t)((uint64_t)id >> 32), a.stream_id),
-        a.key);
-    const uint32_t word[4] = {w.x, w.y, w.z, w.w};
-    const T *x = static_cast<const T *>(a.x) + row * a.sx;
-    const T *r = a.residual ? static_cast<const T *>(a.residual) + row * a.sr : nullptr;
-    T *y = static_cast<T *>(a.y) + row * a.sy;
+// Bit j: column j of the group is kept.
+__device__ __forceinline__ uint32_t keep_bits(const DropoutArgs &a, int64_t id, uint32_t group) {
+  const uint4 w = philox4x32_10(
+      make_uint4(group, (uint32_t)id, (uint32_t)((uint64_t)id >> 32), a.stream_id), a.key);
+  const uint32_t word[4] = {w.x, w.y, w.z, w.w};
+  uint32_t bits = 0;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int col = g * 8 + j;
-      if (col >= a.D) break;
-      const uint32_t lane = (word[j / 2] >> (16 * (j & 1))) & 0xffffu;
-      float v = lane >= a.drop ? to_f32(x[col]) * a.scale : 0.0f;
-      if (r) v += to_f32(r[col]);
-      y[col] = from_f32<T>(v);
+  for (int j = 0; j < 4; ++j) {
+    bits |= ((word[j] & 0xffffu) >= a.drop ? 1u : 0u) << (2 * j);
+    bits |= ((word[j] >> 16) >= a.drop ? 2u : 0u) << (2 * j);
+  }
+  return bits;
+}
+__device__ __forceinline__ uint32_t quotient(const DropoutArgs &a, uint32_t e) {
+  return a.groups == 1 ? e : __umulhi(e, a.magic) >> a.shift;
+}
+
+// Whole groups of eight columns on 16-byte boundaries: a thread per group, one
+// generator call and 16-byte accesses (two where elements have four bytes), two
+// groups in flight.  The generator is about 60 of the 130 issue slots of a group,
+// so that 16-bit data without a residual is bound by them and by memory alike.
+// 24576 x 512 bf16 with a residual: 14.0 us (5.4 TB/s); a thread per group with
+// scalar accesses took 35.5.
+template <typename T, bool RES>
+__global__ void __launch_bounds__(256) dropout_vec_kernel(const __grid_constant__ DropoutArgs a) {
+  constexpr int H = 16 / (int)sizeof(T), PARTS = 8 / H, U = 2;
+  const uint32_t total = (uint32_t)(a.N * a.groups), pace = gridDim.x * 256;
+  for (uint32_t e0 = blockIdx.x * 256 + threadIdx.x; e0 < total; e0 += U * pace) {
+    Raw<T, H> x[U][PARTS], r[U][PARTS];
+    uint32_t row[U], group[U];
+    int64_t id[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const uint32_t e = e0 + u * pace;
+      if (e >= total) break;
+      row[u] = quotient(a, e);
+      group[u] = e - row[u] * a.groups;
+      id[u] = a.rows ? a.rows[row[u]] : a.row0 + row[u];
+      const T *xp = static_cast<const T *>(a.x) + (int64_t)row[u] * a.sx + group[u] * 8;
+      const T *rp = static_cast<const T *>(a.residual) + (int64_t)row[u] * a.sr + group[u] * 8;
+#pragma unroll
+      for (int i = 0; i < PARTS; ++i) {
+        x[u][i] = *reinterpret_cast<const Raw<T, H> *>(xp + i * H);
+        if (RES) r[u][i] = *reinterpret_cast<const Raw<T, H> *>(rp + i * H);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (e0 + u * pace >= total) break;
+      const uint32_t bits = keep_bits(a, id[u], group[u]);
+      T *yp = static_cast<T *>(a.y) + (int64_t)row[u] * a.sy + group[u] * 8;
+#pragma unroll
+      for (int i = 0; i < PARTS; ++i) {
+        Vec<H> v = mul(values<T, H>(x[u][i]), a.scale);
+#pragma unroll
+        for (int j = 0; j < H; ++j) v[j] = bits >> (i * H + j) & 1 ? v[j] : 0.0f;
+        if (RES) v = add(v, values<T, H>(r[u][i]));
+        store_vec<T, H>(yp + i * H, v.v);
+      }
+    }
+  }
+}
+
+// Any width, stride and alignment: a warp per row and segment of 256 columns.
+// Lane l draws group l; column k * 32 + l of the segment takes its bit from the
+// lane that has its group, so every access is to 32 neighbouring elements.
+// 98304 x 333 f32: 55 us (4.8 TB/s); a thread per group took 146.
+template <typename T>
+__global__ void __launch_bounds__(256) dropout_kernel(const __grid_constant__ DropoutArgs a) {
+  const uint32_t lane = threadIdx.x & 31, total = (uint32_t)(a.N * a.groups);
+  for (uint32_t e = blockIdx.x * 8 + (threadIdx.x >> 5); e < total; e += gridDim.x * 8) {
+    const uint32_t row = quotient(a, e), segment = e - row * a.groups;
+    const int64_t id = a.rows ? a.rows[row] : a.row0 + row;
+    const int c0 = segment * 256 + lane;
+    const T *x = static_cast<const T *>(a.x) + (int64_t)row * a.sx + c0;
+    const T *r = static_cast<const T *>(a.residual) + (int64_t)row * a.sr + c0;
+    T *y = static_cast<T *>(a.y) + (int64_t)row * a.sy + c0;
+    T xv[8], rv[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      if (c0 + k * 32 < a.D) {
+        xv[k] = x[k * 32];
+        if (a.residual) rv[k] = r[k * 32];
+      }
+    }
+    const uint32_t mine = keep_bits(a, id, segment * 32 + lane);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const uint32_t bits = __shfl_sync(0xffffffffu, mine, k * 4 + (lane >> 3));
+      if (c0 + k * 32 < a.D) {
+        float v = bits >> (lane & 7) & 1 ? to_f32(xv[k]) * a.scale : 0.0f;
+        if (a.residual) v += to_f32(rv[k]);
+        y[k * 32] = from_f32<T>(v);
+      }
     }
   }
 }
@@ -80,18 +152,39 @@ extern "C" zrl_status zrl_dropout(const void *x, const void *residual, const int
   a.sy = strides ? strides[2] : D;
   if (N > 1 && a.sy < D && a.sy > -D)
     return seq_fail(ZRL_INVALID_ARG, "dropout: rows of y overlap");
-  a.N = N;
   a.D = (int32_t)D;
-  a.groups = (int32_t)((D + 7) / 8);
   const double drop = nearbyint(65536.0 * p);
   a.drop = (uint32_t)drop;
   a.scale = drop < 65536.0 ? (float)(65536.0 / (65536.0 - drop)) : 0.0f;
   a.key = make_uint2((uint32_t)seed, (uint32_t)(seed >> 32));
   a.stream_id = stream_id;
-  const int64_t blocks = std::min<int64_t>((N * a.groups + 255) / 256, 148 * 32);
-  with_dtype(dtype, [&](auto t) {
-    dropout_kernel<decltype(t)>
-        <<<(unsigned)blocks, 256, 0, static_cast<cudaStream_t>(stream)>>>(a);
-  });
+  bool vec = D % 8 == 0 && aligned(x, 16) && aligned(y, 16) && aligned(residual, 16);
+  for (int64_t st : {a.sx, residual ? a.sr : a.sx, a.sy}) vec = vec && (N == 1 || st * es % 16 == 0);
+  a.groups = (int32_t)(vec ? D / 8 : (D + 255) / 256);
+  while ((1u << a.shift) < (uint32_t)a.groups) ++a.shift;
+  a.shift = a.shift ? a.shift - 1 : 0;
+  a.magic = (uint32_t)((((uint64_t)1 << (32 + a.shift)) + a.groups - 1) / a.groups);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  // launches of fewer than 2^31 groups
+  const int64_t most = std::max<int64_t>(1, (((int64_t)1 << 31) - 1) / a.groups);
+  for (int64_t n0 = 0; n0 < N; n0 += most) {
+    a.N = std::min(most, N - n0);
+    a.row0 = n0;
+    const int64_t units = vec ? (a.N * a.groups + 255) / 256 : (a.N * a.groups + 7) / 8;
+    const unsigned blocks = (unsigned)std::min<int64_t>(units, 148 * (vec ? 4 : 16));
+    with_dtype(dtype, [&](auto t) {
+      using T = decltype(t);
+      if (!vec) dropout_kernel<T><<<blocks, 256, 0, st>>>(a);
+      else if (residual) dropout_vec_kernel<T, true><<<blocks, 256, 0, st>>>(a);
+      else dropout_vec_kernel<T, false><<<blocks, 256, 0, st>>>(a);
+    });
+    auto on = [&](auto &ptr, int64_t elements, int size) {
+      if (ptr) ptr = (std::remove_reference_t<decltype(ptr)>)((char *)ptr + elements * size);
+    };
+    on(a.x, most * a.sx, es);
+    on(a.residual, most * a.sr, es);
+    on(a.y, most * a.sy, es);
+    on(a.rows, most, 8);
+  }
   return seq_launched("dropout");
 }

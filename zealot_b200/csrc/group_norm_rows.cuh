@@ -15,10 +15,10 @@ namespace {
 #define RB 2
 #endif
 #ifndef TB
-#define TB 4
+#define TB 6
 #endif
 #ifndef TGB
-#define TGB 3
+#define TGB 4
 #endif
 constexpr int kLaneBlocks = RB;  // resident blocks of the lanes form
 
