@@ -9,7 +9,6 @@
 // The kernels are in group_norm_rows.cuh (L = 1) and group_norm_samples.cuh;
 // here a call is checked and laid out.
 #include <math.h>
-#include <string.h>
 
 #include <algorithm>
 #include <initializer_list>
@@ -22,12 +21,6 @@
 namespace zrl {
 namespace {
 
-#ifndef FSAMP
-#define FSAMP 2
-#endif
-#ifndef GSAMP
-#define GSAMP 2
-#endif
 constexpr int64_t kBatchBytes = 110 << 20;  // of two passes that meet in L2
 constexpr int64_t kBlockBytes = 64 << 10;   // shared memory of the block form
 
@@ -52,40 +45,38 @@ struct ParamOut {
   }
 };
 
-// Whether a call's tensors can be taken in vectors, and in one run.
+// A call, and whether its tensors can be taken in vectors.
 struct NormShape {
   int64_t N, L, C;
   int32_t G;
   int es;
   bool grad;
   int64_t align;       // bytes that pointers and strides are multiples of: 16, 8, 4 or es
-  bool flat;           // rows without gaps between them, from 16-byte boundaries on
   int64_t row_stride;  // the largest
 };
 
 // How a call is laid out.
-//  lanes:   L = 1 and the group is whole vectors of 4 to 16 bytes: E vectors a
-//           lane, p lanes a group.  Eight channels a lane where the group has
-//           them, so that the shuffles of the sums are shared by as many.
-//  tiles:   L = 1, any other width, dense rows.
+//  lanes:   L = 1: E vectors of 16 bytes to one element a lane, p lanes a
+//           group.  About eight channels a lane where the group has them, so
+//           that the shuffles of the sums are shared by as many: at w = 25 in
+//           fp32, four by eight lanes took 71 us, one by 32 lanes 92 us
+//           (98304 x 250 forward).
 //  block:   a sample's columns fit a block's shared memory.
 //  passes:  the rest.
 struct NormPlan {
-  enum { kLanes, kTiles, kBlock, kPasses } form;
-  int vec, E, p, gb, rb, blocks, across;  // lanes and tiles
+  enum { kLanes, kBlock, kPasses } form;
+  int vec, E, p, gb, rb, blocks, across;  // lanes
   int cols, parts, stretches, depth;      // samples (depth: blocks over channels)
   int64_t stretch, batch, bytes;          // batch: samples of a launch; shared memory
 };
 
 bool plan_lanes(const NormShape &s, NormPlan *p) {
   const int64_t w = s.C / s.G;
-  int vec = 0;
-  for (int bytes = 16; bytes >= 4 && !vec; bytes /= 2)
-    if (bytes / s.es >= 2 && s.align % bytes == 0 && w % (bytes / s.es) == 0) vec = bytes / s.es;
-  if (!vec) return false;
+  int vec = 16 / s.es;
+  while (w % vec || s.align % (vec * s.es)) vec /= 2;
   const int64_t nv = w / vec, most = vec >= 4 ? 2 : 4;
   int64_t E = 1;
-  while (E < most && E * vec < 8 && E < nv) E *= 2;
+  while (E < most && E * vec < 8 && 8 * E < nv) E *= 2;
   while (E < most && (nv + E - 1) / E > 32) E *= 2;
   if ((nv + E - 1) / E > 32) return false;
   p->form = NormPlan::kLanes;
@@ -101,26 +92,6 @@ bool plan_lanes(const NormShape &s, NormPlan *p) {
   p->blocks = (int)std::max<int64_t>(
       1, std::min<int64_t>((s.N + p->rb - 1) / p->rb, kSms * kLaneBlocks / p->across));
   return s.row_stride <= INT32_MAX / ((int64_t)p->rb * s.es) && p->across <= 65535;
-}
-
-int64_t tile_smem(const NormShape &s, int rb) {
-  const int64_t tile = s.es == 2 ? tile_elements<__half>() : tile_elements<float>();
-  return 4 * (s.grad ? 2 * tile + 4 * s.C + 2 * (int64_t)rb * s.G : tile + 2 * s.C);
-}
-
-bool plan_tiles(const NormShape &s, NormPlan *p) {
-  const int64_t tile = s.es == 2 ? tile_elements<__half>() : tile_elements<float>();
-  const int64_t rb = (tile - 16 / s.es) / s.C;
-  if (!s.flat || rb < 1) return false;
-  p->form = NormPlan::kTiles;
-  const int64_t resident = s.grad ? TGB : TB;
-  // enough tiles for the resident blocks
-  p->rb = (int)std::min<int64_t>(rb, (s.N + kSms * resident - 1) / (kSms * resident));
-  p->p = 1;
-  while (p->p < 32 && 2 * p->p * p->rb * s.G <= kThreads && p->p < s.C / s.G) p->p *= 2;
-  p->blocks = (int)std::min<int64_t>((s.N + p->rb - 1) / p->rb, kSms * resident);
-  p->bytes = tile_smem(s, p->rb);
-  return p->bytes <= 160 << 10;
 }
 
 // Channels of a block: the whole row where it fits, else as many groups as make
@@ -153,8 +124,7 @@ bool plan_columns(const NormShape &s, int vec, int64_t most_channels, NormPlan *
 NormPlan plan_samples(const NormShape &s) {
   NormPlan p{};
   const int64_t tensors = s.grad ? 2 : 1;
-  for (int bytes = 16; bytes >= s.es; bytes /= 2) {
-    const int vec = bytes / s.es;
+  for (int vec = std::min(16 / s.es, MAXV); vec >= 1; vec /= 2) {
     if (!plan_columns(s, vec, (int64_t)kThreads * vec, &p)) continue;
     // the block form, with columns of 128 bytes or the group if it is wider
     NormPlan b = p;
@@ -177,7 +147,7 @@ NormPlan plan_samples(const NormShape &s) {
     // one wave of the resident blocks, and some positions for each thread
     const int64_t rows = kThreads / (p.cols / vec);
     const int64_t want =
-        std::max<int64_t>(1, kSms * (s.grad ? GSAMP : FSAMP) / (p.batch * p.depth));
+        std::max<int64_t>(1, kSms * (vec <= 4 ? s.grad ? SGB4 : SB4 : 2) / (p.batch * p.depth));
     const int64_t fit = std::max<int64_t>(1, s.L / (rows * 4));
     p.stretches = (int)std::max<int64_t>(1, std::min<int64_t>({want, fit, (int64_t)512}));
     p.stretch = ((s.L + p.stretches - 1) / p.stretches + rows * 4 - 1) / (rows * 4) * (rows * 4);
@@ -190,13 +160,11 @@ NormPlan plan_samples(const NormShape &s) {
 NormPlan plan_norm(const NormShape &s) {
   NormPlan p{};
   if (s.L == 1 && plan_lanes(s, &p)) return p;
-  p = NormPlan{};
-  if (s.L == 1 && plan_tiles(s, &p)) return p;
   return plan_samples(s);
 }
 
 int64_t workspace_floats(const NormPlan &p, const NormShape &s) {
-  if (p.form == NormPlan::kLanes || p.form == NormPlan::kTiles)
+  if (p.form == NormPlan::kLanes)
     return s.grad ? (int64_t)p.blocks * 2 * s.C : 0;
   if (s.grad)
     return s.N * p.stretches * 2 *
@@ -217,11 +185,9 @@ void with_vec(int32_t dtype, int vec, F &&f) {
 }
 template <int VEC, typename F>
 void with_e(int E, F &&f) {
-  if constexpr (VEC > 1) {
-    if (E == 1) f(std::integral_constant<int, 1>{});
-    else if (E == 2) f(std::integral_constant<int, 2>{});
-    else if constexpr (VEC == 2) f(std::integral_constant<int, 4>{});
-  }
+  if (E == 1) f(std::integral_constant<int, 1>{});
+  else if (E == 2) f(std::integral_constant<int, 2>{});
+  else if constexpr (VEC <= 2) f(std::integral_constant<int, 4>{});
 }
 
 void use_plan(NormArgs &a, const NormPlan &p, void *workspace) {
@@ -264,14 +230,12 @@ void launch_norm(void (*kernel)(NormArgs), dim3 grid, const NormPlan &p, cudaStr
 // What the call's pointers and strides allow.
 NormShape shape_of(const NormArgs &a, int es, bool grad,
                    std::initializer_list<const void *> ptrs) {
-  NormShape s{a.N, a.L, a.C, a.G, es, grad, 16, true, 1};
+  NormShape s{a.N, a.L, a.C, a.G, es, grad, 16, 1};
   for (const void *p : ptrs)
     while (!aligned(p, s.align)) s.align /= 2;
-  s.flat = s.align == 16;
   for (int64_t t : {a.sxn, a.syn, grad ? a.sdn : a.syn}) {
     if (a.N > 1) {
       while (t * es % s.align) s.align /= 2;
-      s.flat = s.flat && t == a.C;
       s.row_stride = std::max(s.row_stride, t < 0 ? -t : t);
     }
   }
@@ -311,11 +275,10 @@ extern "C" int64_t zrl_group_norm_workspace(int64_t N, int64_t L, int64_t C, int
   int64_t most = 0;
   for (int es : {2, 4})
     for (int64_t align = 16; align >= es; align /= 2)
-      for (bool flat : {true, false})
-        for (int64_t row_stride : {(int64_t)1, INT64_MAX}) {
-          const NormShape s{N, L, C, groups, es, grad != 0, align, flat, row_stride};
-          most = std::max(most, workspace_floats(plan_norm(s), s));
-        }
+      for (int64_t row_stride : {(int64_t)1, INT64_MAX}) {
+        const NormShape s{N, L, C, groups, es, grad != 0, align, row_stride};
+        most = std::max(most, workspace_floats(plan_norm(s), s));
+      }
   return most * (int64_t)sizeof(float);
 }
 
@@ -363,12 +326,6 @@ extern "C" zrl_status zrl_group_norm(const void *x, const float *gamma, const fl
   if (workspace_bytes < need || !aligned(workspace, 16) || (!workspace && need))
     return seq_fail(ZRL_INVALID_ARG, "group_norm: workspace too small or not aligned");
   use_plan(a, p, workspace);
-  if (p.form == NormPlan::kTiles) {
-    with_dtype(dtype, [&](auto t) {
-      launch_norm(norm_tile_kernel<decltype(t)>, dim3((unsigned)p.blocks), p, st, a);
-    });
-    return seq_launched("group_norm");
-  }
   with_vec(dtype, p.vec, [&](auto t, auto v) {
     using T = decltype(t);
     constexpr int VEC = decltype(v)::value;
@@ -443,36 +400,29 @@ extern "C" zrl_status zrl_group_norm_grad(const void *x, const void *dy, const f
     return seq_fail(ZRL_INVALID_ARG, "group_norm_grad: workspace too small");
   use_plan(a, p, workspace);
   int64_t sums = N * p.stretches;  // rows of channel sums
-  if (p.form == NormPlan::kTiles) {
-    with_dtype(dtype, [&](auto t) {
-      launch_norm(norm_tile_grad_kernel<decltype(t)>, dim3((unsigned)p.blocks), p, st, a);
-    });
-    sums = p.blocks;
-  } else {
-    with_vec(dtype, p.vec, [&](auto t, auto v) {
-      using T = decltype(t);
-      constexpr int VEC = decltype(v)::value;
-      if (p.form == NormPlan::kLanes) {
-        with_e<VEC>(p.E, [&](auto e) {
-          norm_rows_grad_kernel<T, VEC, decltype(e)::value>
-              <<<dim3((unsigned)p.blocks, (unsigned)p.across), kThreads, 0, st>>>(a);
-        });
-        sums = p.blocks;
-        return;
+  with_vec(dtype, p.vec, [&](auto t, auto v) {
+    using T = decltype(t);
+    constexpr int VEC = decltype(v)::value;
+    if (p.form == NormPlan::kLanes) {
+      with_e<VEC>(p.E, [&](auto e) {
+        norm_rows_grad_kernel<T, VEC, decltype(e)::value>
+            <<<dim3((unsigned)p.blocks, (unsigned)p.across), kThreads, 0, st>>>(a);
+      });
+      sums = p.blocks;
+      return;
+    }
+    for (int64_t n0 = 0; n0 < N; n0 += p.batch) {
+      const NormArgs b = samples_from(a, n0, es);
+      const dim3 grid((unsigned)p.stretches, (unsigned)std::min(p.batch, N - n0),
+                      (unsigned)p.depth);
+      if (p.form == NormPlan::kBlock) {
+        launch_norm(norm_block_grad_kernel<T, VEC>, grid, p, st, b);
+        continue;
       }
-      for (int64_t n0 = 0; n0 < N; n0 += p.batch) {
-        const NormArgs b = samples_from(a, n0, es);
-        const dim3 grid((unsigned)p.stretches, (unsigned)std::min(p.batch, N - n0),
-                        (unsigned)p.depth);
-        if (p.form == NormPlan::kBlock) {
-          launch_norm(norm_block_grad_kernel<T, VEC>, grid, p, st, b);
-          continue;
-        }
-        norm_grad_sums_kernel<T, VEC><<<grid, kThreads, 0, st>>>(b);
-        norm_grad_apply_kernel<T, VEC><<<grid, kThreads, 0, st>>>(b);
-      }
-    });
-  }
+      norm_grad_sums_kernel<T, VEC><<<grid, kThreads, 0, st>>>(b);
+      norm_grad_apply_kernel<T, VEC><<<grid, kThreads, 0, st>>>(b);
+    }
+  });
   launch_column_sum(a.part, sums, 2 * C, ParamOut{dgamma, dbeta, C}, st);
   return seq_launched("group_norm_grad");
 }

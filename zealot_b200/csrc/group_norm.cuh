@@ -21,7 +21,7 @@ struct NormArgs {
   float eps;
   bool wide;    // gamma and beta start on 16 bytes
   int32_t one;  // 1
-  // lanes and tiles: lanes per group; groups of a block, rows of a block or tile
+  // rows: lanes per group, groups of a block, rows of a block
   int32_t p, gb, rb;
   // samples: channels of a block at most, parts of a wide group, stretches of
   // positions, positions of one

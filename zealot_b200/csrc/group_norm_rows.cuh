@@ -1,9 +1,6 @@
-// group_norm_rows.cuh -- group norm of rows by themselves (L = 1).
-//
-// Two forms, both one pass over the data with the next rows' loads in flight.
-// Lanes: a group's channels are whole vectors, held in registers by a few lanes
-// next to one another in a warp.  Tiles: any other width; a tile of rows goes
-// through shared memory, in and out as a flat run of 16-byte vectors.
+// group_norm_rows.cuh -- group norm of rows by themselves (L = 1): one pass, a
+// group's channels in the registers of a few lanes next to one another in a
+// warp, the next rows' loads in flight.
 #pragma once
 
 #include "group_norm.cuh"
@@ -11,16 +8,7 @@
 namespace zrl {
 namespace {
 
-#ifndef RB
-#define RB 2
-#endif
-#ifndef TB
-#define TB 6
-#endif
-#ifndef TGB
-#define TGB 4
-#endif
-constexpr int kLaneBlocks = RB;  // resident blocks of the lanes form
+constexpr int kLaneBlocks = 2;  // resident blocks
 
 // A thread of the row form: E vectors of VEC channels of one group, the same
 // ones in every row it meets, so its gammas and betas stay in registers.
@@ -169,35 +157,35 @@ __global__ void __launch_bounds__(kThreads, kLaneBlocks)
   for (int e = 0; e < E; ++e) dg[e] = db[e] = all<VEC>(0.0f);
   const int64_t pace = (int64_t)gridDim.x * a.rb * U;
   int64_t n = (int64_t)blockIdx.x * a.rb * U + k.r;
-  RowPlaces<T, E> xs(a.x, a.sxn, k.at, n, a, U), ds(a.dy, a.syn, k.at, n, a, U),
-      os(a.dx, a.sdn, k.at, n, a, U);
+  // rows follow by adding strides; a vector's offset is added at each access
+  const T *x0 = static_cast<const T *>(a.x) + n * a.sxn;
+  const T *d0 = static_cast<const T *>(a.dy) + n * a.syn;
+  T *o0 = static_cast<T *>(a.dx) + n * a.sdn;
+  const int64_t xu = a.rb * a.sxn, du = a.rb * a.syn, ou = a.rb * a.sdn;
   Raw<T, VEC> rx[U][E], rd[U][E];
   float mu[U], rstd[U];
   auto load = [&](int64_t first) {
+    const T *xr = x0, *dr = d0;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
+    for (int u = 0; u < U; ++u, xr += xu, dr += du) {
       const int64_t row = first + u * a.rb;
-      if (row < a.N) {
 #pragma unroll
-        for (int e = 0; e < E; ++e)
-          if (k.has[e]) {
-            rx[u][e] = *reinterpret_cast<const Raw<T, VEC> *>(xs.p[e]);
-            rd[u][e] = *reinterpret_cast<const Raw<T, VEC> *>(ds.p[e]);
-          }
-        if (k.on) {
-          mu[u] = a.mean[row * a.G + k.g];
-          rstd[u] = a.rstd[row * a.G + k.g];
+      for (int e = 0; e < E; ++e)
+        if (row < a.N && k.has[e]) {
+          rx[u][e] = *reinterpret_cast<const Raw<T, VEC> *>(xr + k.at[e]);
+          rd[u][e] = *reinterpret_cast<const Raw<T, VEC> *>(dr + k.at[e]);
         }
+      if (row < a.N && k.on) {
+        mu[u] = a.mean[row * a.G + k.g];
+        rstd[u] = a.rstd[row * a.G + k.g];
       } else {  // adds nothing to any sum
 #pragma unroll
         for (int e = 0; e < E; ++e) rx[u][e] = rd[u][e] = Raw<T, VEC>{};
         mu[u] = 0.0f, rstd[u] = 0.0f;
       }
-      xs.next_row(a.one);
-      ds.next_row(a.one);
     }
-    xs.next_turn();
-    ds.next_turn();
+    x0 += pace * a.sxn;
+    d0 += pace * a.syn;
   };
 #pragma unroll
   for (int u = 0; u < U; ++u) {
@@ -231,19 +219,18 @@ __global__ void __launch_bounds__(kThreads, kLaneBlocks)
     load(n + pace);
     lanes_sum(s1, a.p);
     lanes_sum(s2, a.p);
+    T *orow = o0;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (n + u * a.rb < a.N) {
-        const float m1 = s1[u] * inv, m2 = s2[u] * inv;
+    for (int u = 0; u < U; ++u, orow += ou) {
+      if (n + u * a.rb >= a.N) break;
+      const float m1 = s1[u] * inv, m2 = s2[u] * inv;
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const Vec<VEC> o = mul(add(d[u][e], fma(x[u][e], -m2, -m1)), rs[u]);
-          if (k.has[e]) store_vec<T, VEC>(os.p[e], o.v);
-        }
+      for (int e = 0; e < E; ++e) {
+        const Vec<VEC> o = mul(add(d[u][e], fma(x[u][e], -m2, -m1)), rs[u]);
+        if (k.has[e]) store_vec<T, VEC>(orow + k.at[e], o.v);
       }
-      os.next_row(a.one);
     }
-    os.next_turn();
+    o0 += pace * a.sdn;
   }
   // the rows of the block, in order
   const int per_row = a.gb * a.p;
@@ -262,240 +249,6 @@ __global__ void __launch_bounds__(kThreads, kLaneBlocks)
           a.part[((int64_t)blockIdx.x * 2 + which) * a.C + k.at[e] + i] = s;
         }
       }
-}
-
-// ---------------------------------------------------------------- tiles
-
-constexpr int kTileVecs = 4;  // 16-byte vectors of a tile a thread and tensor
-template <typename T>
-constexpr int tile_elements() { return kTileVecs * kThreads * (16 / (int)sizeof(T)); }
-
-// A tile of rb rows of a dense [N, C] tensor as whole 16-byte vectors: from the
-// vector that its first element lies in to the one of its last.  The vectors at
-// the two ends may hold elements of the neighbours, which are read and not used,
-// and are written element by element.
-template <typename T>
-struct TileSpan {
-  static constexpr int VEC = 16 / (int)sizeof(T);
-  int64_t begin, start, end;  // elements; start: begin rounded down to a vector
-  int rows;
-  __device__ __forceinline__ TileSpan(const NormArgs &a, int64_t tile) {
-    rows = (int)min((int64_t)a.rb, a.N - tile * a.rb);
-    begin = tile * a.rb * a.C;
-    start = begin / VEC * VEC;
-    end = begin + (int64_t)rows * a.C;
-  }
-  __device__ __forceinline__ int64_t at(int v) const {
-    return start + (int64_t)(v * kThreads + threadIdx.x) * VEC;
-  }
-  __device__ __forceinline__ void load(const void *p, int64_t total,
-                                       Raw<T, VEC> (&raw)[kTileVecs]) const {
-    const T *x = static_cast<const T *>(p);
-#pragma unroll
-    for (int v = 0; v < kTileVecs; ++v) {
-      const int64_t f = at(v);
-      if (f + VEC <= total && f < end) {
-        raw[v] = *reinterpret_cast<const Raw<T, VEC> *>(x + f);
-      } else if (f < end) {
-        T e[VEC];
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) e[i] = f + i < total ? x[f + i] : T{};
-        memcpy(&raw[v], e, sizeof(raw[v]));
-      }
-    }
-  }
-  __device__ __forceinline__ void put(const Raw<T, VEC> (&raw)[kTileVecs], float *s) const {
-#pragma unroll
-    for (int v = 0; v < kTileVecs; ++v) {
-      if (at(v) >= end) break;
-      float e[VEC];
-      unpack<T, VEC>(raw[v], e);
-      float4 *to = reinterpret_cast<float4 *>(s + (v * kThreads + threadIdx.x) * VEC);
-#pragma unroll
-      for (int i = 0; i < VEC; i += 4) to[i / 4] = make_float4(e[i], e[i + 1], e[i + 2], e[i + 3]);
-    }
-  }
-  __device__ __forceinline__ void store(void *p, const float *s) const {
-    T *y = static_cast<T *>(p);
-#pragma unroll
-    for (int v = 0; v < kTileVecs; ++v) {
-      const int64_t f = at(v);
-      if (f >= end) break;
-      float e[VEC];
-      const float4 *from = reinterpret_cast<const float4 *>(s + (v * kThreads + threadIdx.x) * VEC);
-#pragma unroll
-      for (int i = 0; i < VEC; i += 4) {
-        const float4 q = from[i / 4];
-        e[i] = q.x, e[i + 1] = q.y, e[i + 2] = q.z, e[i + 3] = q.w;
-      }
-      if (f >= begin && f + VEC <= end) {
-        store_vec<T, VEC>(y + f, e);
-      } else {
-#pragma unroll
-        for (int i = 0; i < VEC; ++i)
-          if (f + i >= begin && f + i < end) y[f + i] = from_f32<T>(e[i]);
-      }
-    }
-  }
-};
-
-// Group r, g of the tile for each p lanes; f(row, group, lane, on) is called by
-// whole warps.
-template <typename F>
-__device__ __forceinline__ void each_group(const NormArgs &a, int rows, F f) {
-  const int count = rows * a.G, at_once = kThreads / a.p, lane = threadIdx.x & (a.p - 1);
-  for (int t0 = 0; t0 < count; t0 += at_once) {
-    const int t = t0 + threadIdx.x / a.p, r = t / a.G;
-    f(r, t - r * a.G, lane, t < count);
-  }
-}
-
-template <typename T>
-__global__ void __launch_bounds__(kThreads, TB)
-    norm_tile_kernel(const __grid_constant__ NormArgs a) {
-  constexpr int VEC = 16 / (int)sizeof(T);
-  float *s = reinterpret_cast<float *>(norm_smem);
-  float *ga = s + tile_elements<T>(), *be = ga + a.C;
-  for (int c = threadIdx.x; c < a.C; c += kThreads) {
-    ga[c] = a.gamma ? a.gamma[c] : 1.0f;
-    be[c] = a.beta ? a.beta[c] : 0.0f;
-  }
-  const int64_t tiles = (a.N + a.rb - 1) / a.rb, total = a.N * a.C;
-  const float inv = 1.0f / (float)a.w;
-  Raw<T, VEC> raw[kTileVecs] = {};
-  int64_t tile = blockIdx.x;
-  if (tile < tiles) TileSpan<T>(a, tile).load(a.x, total, raw);
-  for (; tile < tiles; tile += gridDim.x) {
-    const TileSpan<T> span(a, tile);
-    span.put(raw, s);
-    __syncthreads();
-    if (tile + gridDim.x < tiles) TileSpan<T>(a, tile + gridDim.x).load(a.x, total, raw);
-    float *own = s + (span.begin - span.start);
-    each_group(a, span.rows, [&](int r, int g, int lane, bool on) {
-      float *x = own + r * a.C + g * a.w;
-      const int w = on ? a.w : 0;
-      float mu[1] = {0.0f}, q[1] = {0.0f};
-#pragma unroll 4
-      for (int j = lane; j < w; j += a.p) mu[0] += x[j];
-      lanes_sum(mu, a.p);
-      mu[0] *= inv;
-#pragma unroll 4
-      for (int j = lane; j < w; j += a.p) {
-        const float d = x[j] - mu[0];
-        q[0] = fmaf(d, d, q[0]);
-      }
-      lanes_sum(q, a.p);
-      const float rstd = rsqrtf(fmaf(q[0], inv, a.eps));
-      const float *gg = ga + g * a.w, *bb = be + g * a.w;
-#pragma unroll 4
-      for (int j = lane; j < w; j += a.p) {
-        Vec<1> z;
-        z[0] = fmaf((x[j] - mu[0]) * rstd, gg[j], bb[j]);
-        act_values<1>(z, a.act);
-        x[j] = z[0];
-      }
-      if (on && lane == 0) {
-        const int64_t ng = (tile * a.rb + r) * a.G + g;
-        if (a.mean) a.mean[ng] = mu[0];
-        if (a.rstd) a.rstd[ng] = rstd;
-      }
-    });
-    __syncthreads();
-    span.store(a.y, s);
-    __syncthreads();
-  }
-}
-
-// dx, and part[block][2][C] as norm_rows_grad_kernel.  In shared memory x becomes
-// xh, then dx; dy becomes dz.
-template <typename T>
-__global__ void __launch_bounds__(kThreads, TGB)
-    norm_tile_grad_kernel(const __grid_constant__ NormArgs a) {
-  constexpr int VEC = 16 / (int)sizeof(T);
-  float *s = reinterpret_cast<float *>(norm_smem), *d = s + tile_elements<T>();
-  float *ga = d + tile_elements<T>(), *be = ga + a.C, *dg = be + a.C, *db = dg + a.C;
-  float *m1 = db + a.C, *m2 = m1 + a.rb * a.G;  // of each group of the tile, by rstd
-  for (int c = threadIdx.x; c < a.C; c += kThreads) {
-    ga[c] = a.gamma ? a.gamma[c] : 1.0f;
-    be[c] = a.beta ? a.beta[c] : 0.0f;
-    dg[c] = db[c] = 0.0f;
-  }
-  const int64_t tiles = (a.N + a.rb - 1) / a.rb, total = a.N * a.C;
-  const float inv = 1.0f / (float)a.w;
-  Raw<T, VEC> rx[kTileVecs] = {}, rd[kTileVecs] = {};
-  int64_t tile = blockIdx.x;
-  if (tile < tiles) {
-    TileSpan<T>(a, tile).load(a.x, total, rx);
-    TileSpan<T>(a, tile).load(a.dy, total, rd);
-  }
-  for (; tile < tiles; tile += gridDim.x) {
-    const TileSpan<T> span(a, tile);
-    span.put(rx, s);
-    span.put(rd, d);
-    __syncthreads();
-    if (tile + gridDim.x < tiles) {
-      const TileSpan<T> next(a, tile + gridDim.x);
-      next.load(a.x, total, rx);
-      next.load(a.dy, total, rd);
-    }
-    const int skip = (int)(span.begin - span.start);
-    each_group(a, span.rows, [&](int r, int g, int lane, bool on) {
-      float *x = s + skip + r * a.C + g * a.w, *dz = d + skip + r * a.C + g * a.w;
-      const float *gg = ga + g * a.w, *bb = be + g * a.w;
-      const int w = on ? a.w : 0;
-      const int64_t ng = (tile * a.rb + r) * a.G + g;
-      const float mu = on ? a.mean[ng] : 0.0f, rstd = on ? a.rstd[ng] : 0.0f;
-      float t1[1] = {0.0f}, t2[1] = {0.0f};
-#pragma unroll 4
-      for (int j = lane; j < w; j += a.p) {
-        const float xh = (x[j] - mu) * rstd;
-        Vec<1> z;
-        z[0] = fmaf(xh, gg[j], bb[j]);
-        act_slopes<1>(z, a.act);
-        const float e = dz[j] * z[0], f = e * gg[j];
-        x[j] = xh;
-        dz[j] = e;
-        t1[0] += f;
-        t2[0] = fmaf(f, xh, t2[0]);
-      }
-      lanes_sum(t1, a.p);
-      lanes_sum(t2, a.p);
-      if (on && lane == 0) {
-        m1[r * a.G + g] = t1[0] * inv * rstd;
-        m2[r * a.G + g] = t2[0] * inv * rstd;
-      }
-    });
-    __syncthreads();
-    for (int c = threadIdx.x; c < a.C; c += kThreads) {
-      float sg = dg[c], sb = db[c];
-#pragma unroll 4
-      for (int r = 0; r < span.rows; ++r) {
-        const float e = d[skip + r * a.C + c];
-        sg = fmaf(e, s[skip + r * a.C + c], sg);
-        sb += e;
-      }
-      dg[c] = sg;
-      db[c] = sb;
-    }
-    __syncthreads();
-    each_group(a, span.rows, [&](int r, int g, int lane, bool on) {
-      if (!on) return;
-      float *x = s + skip + r * a.C + g * a.w;
-      const float *dz = d + skip + r * a.C + g * a.w, *gg = ga + g * a.w;
-      const float rstd = a.rstd[(tile * a.rb + r) * a.G + g];
-      const float n1 = m1[r * a.G + g], n2 = m2[r * a.G + g];
-#pragma unroll 4
-      for (int j = lane; j < a.w; j += a.p)
-        x[j] = fmaf(dz[j] * gg[j], rstd, -fmaf(x[j], n2, n1));
-    });
-    __syncthreads();
-    span.store(a.dx, s);
-    __syncthreads();
-  }
-  for (int c = threadIdx.x; c < a.C; c += kThreads) {
-    a.part[((int64_t)blockIdx.x * 2) * a.C + c] = dg[c];
-    a.part[((int64_t)blockIdx.x * 2 + 1) * a.C + c] = db[c];
-  }
 }
 
 }  // namespace

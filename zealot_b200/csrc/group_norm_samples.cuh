@@ -13,9 +13,19 @@
 namespace zrl {
 namespace {
 
-#ifndef SB
-#define SB 2
+#ifndef SB4
+#define SB4 4
 #endif
+#ifndef SGB4
+#define SGB4 3
+#endif
+#ifndef MAXV
+#define MAXV 4
+#endif
+// Blocks an SM holds, which bounds their registers.
+template <int VEC, bool GRAD> constexpr int sample_blocks() {
+  return VEC <= 4 ? GRAD ? SGB4 : SB4 : 2;
+}
 
 // A block's channels (whole groups, or a part of one wide group) and positions.
 template <int VEC>
@@ -160,55 +170,69 @@ struct Spread {
     m2 = add(m2, fma(mul(d, d), cnt * share, q));
     cnt = total;
   }
-  template <typename T, int U>
-  __device__ __forceinline__ void take_batch(const Raw<T, VEC> (&raw)[U][1], int count) {
-    if (count == U) {
-      Vec<VEC> v[U];
+  // the values of a turn of each_position
+  template <typename T, int U, typename R>
+  __device__ __forceinline__ void take_turn(const Raw<T, VEC> (&raw)[U][1], int count, R reload) {
+    Vec<VEC> v[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) v[u] = values<T, VEC>(raw[u][0]);
+    for (int u = 0; u < U; ++u) v[u] = values<T, VEC>(raw[u][0]);
+    reload();
+    if (count == U) {
       take(v);
     } else {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         if (u >= count) break;
-        Vec<VEC> v[1] = {values<T, VEC>(raw[u][0])};
-        take(v);
+        Vec<VEC> one[1] = {v[u]};
+        take(one);
       }
     }
   }
 };
 
-// f(position, slot, raw, count) over the thread's positions of TENSORS tensors,
-// slot counting them; U positions are loaded at a time, the next ones while the
-// present ones are worked on.
+// A thread's places in one tensor: its channels at its first position, and the
+// bytes from one of its positions to the next.
+template <typename T>
+struct Run {
+  T *p;
+  int64_t step;
+  template <int VEC>
+  __device__ __forceinline__ Run(const void *base, const Patch<VEC> &k, int64_t sn, int64_t sl)
+      : p(const_cast<T *>(static_cast<const T *>(base)) + k.n * sn + (k.l0 + k.row) * sl +
+          k.channel()),
+        step(k.rows * sl * (int64_t)sizeof(T)) {}
+  __device__ __forceinline__ void next() { p = (T *)((char *)p + step); }
+};
+
+// f(raw, count, reload) over the thread's positions, U at a time (count of them in
+// the last turn); f calls reload() when it is done with raw, so that the next
+// ones' loads are in flight while it works.
 template <int U, typename T, int VEC, int TENSORS, typename F>
-__device__ __forceinline__ void each_position(const Patch<VEC> &k, const T *const (&base)[TENSORS],
-                                              const int64_t (&stride)[TENSORS], F f) {
+__device__ __forceinline__ void each_position(const Patch<VEC> &k, Run<T> (&x)[TENSORS], F f) {
   Raw<T, VEC> raw[U][TENSORS];
-  auto load = [&](int64_t l) {
+  int left = k.on ? (int)((k.l1 - k.l0 - k.row + k.rows - 1) / k.rows) : 0;
+  auto load = [&](int n) {
+    if (n >= U) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int64_t at = l + (int64_t)u * k.rows;
-      if (at < k.l1) {
+      for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int i = 0; i < TENSORS; ++i)
-          raw[u][i] = *reinterpret_cast<const Raw<T, VEC> *>(base[i] + at * stride[i]);
-      }
+        for (int i = 0; i < TENSORS; ++i) {
+          raw[u][i] = *reinterpret_cast<const Raw<T, VEC> *>(x[i].p);
+          x[i].next();
+        }
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (u < n)
+#pragma unroll
+          for (int i = 0; i < TENSORS; ++i) {
+            raw[u][i] = *reinterpret_cast<const Raw<T, VEC> *>(x[i].p);
+            x[i].next();
+          }
     }
   };
-  int64_t l = k.l0 + k.row;
-  load(l);
-  for (int slot = 0; l < k.l1; slot += U) {
-    Raw<T, VEC> now[U][TENSORS];
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int i = 0; i < TENSORS; ++i) now[u][i] = raw[u][i];
-    const int64_t at = l;
-    l += (int64_t)U * k.rows;
-    load(l);
-    f(at, slot, now, (int)min((int64_t)U, (k.l1 - at + k.rows - 1) / k.rows));
-  }
+  load(left);
+  for (; left > 0; left -= U) f(raw, min(left, U), [&]() { load(left - U); });
 }
 
 template <typename T, int VEC>
@@ -229,19 +253,15 @@ __device__ __forceinline__ void block_spread(const Patch<VEC> &k, const Spread<V
 // First pass: part[n][group][piece] = (mean, squares about it) of the block's
 // piece.
 template <typename T, int VEC>
-__global__ void __launch_bounds__(kThreads, SB)
+__global__ void __launch_bounds__(kThreads, (sample_blocks<VEC, false>()))
     norm_stats_kernel(const __grid_constant__ NormArgs a) {
   __shared__ Sums<T, VEC> buf, mu, m2;
   const Patch<VEC> k(a);
   Spread<VEC> t;
-  if (k.on) {
-    const T *const base[1] = {static_cast<const T *>(a.x) + k.n * a.sxn + k.channel()};
-    const int64_t stride[1] = {a.sxl};
-    each_position<4, T, VEC, 1>(k, base, stride,
-                                [&](int64_t, int, Raw<T, VEC>(&raw)[4][1], int count) {
-                                  t.template take_batch<T, 4>(raw, count);
-                                });
-  }
+  Run<T> x[1] = {Run<T>(a.x, k, a.sxn, a.sxl)};
+  each_position<4, T, VEC, 1>(k, x, [&](Raw<T, VEC>(&raw)[4][1], int count, auto reload) {
+    t.template take_turn<T, 4>(raw, count, reload);
+  });
   block_spread(k, t, (float)(k.l1 - k.l0) * (float)k.per, buf, mu, m2);
   const int pieces = a.stretches * a.parts, piece = blockIdx.x * a.parts + k.part;
   float2 *p = reinterpret_cast<float2 *>(a.part);
@@ -260,8 +280,8 @@ struct Scale {
     be = params<VEC>(a.beta, k.channel(), 0.0f, a.wide);
   }
   template <typename T>
-  __device__ __forceinline__ void write(const Raw<T, VEC> &raw, int act, T *y) const {
-    Vec<VEC> z = fma(add(values<T, VEC>(raw), mu), gr, be);
+  __device__ __forceinline__ void write(const Vec<VEC> &x, int act, T *y) const {
+    Vec<VEC> z = fma(add(x, mu), gr, be);
     act_values<VEC>(z, act);
     store_vec<T, VEC>(y, z.v);
   }
@@ -269,7 +289,7 @@ struct Scale {
 
 // Second pass: the pieces' means and squares give the group's, then y.
 template <typename T, int VEC>
-__global__ void __launch_bounds__(kThreads, SB)
+__global__ void __launch_bounds__(kThreads, (sample_blocks<VEC, false>()))
     norm_apply_kernel(const __grid_constant__ NormArgs a) {
   __shared__ Sums<T, VEC> mean, rstd;
   const Patch<VEC> k(a);
@@ -301,18 +321,19 @@ __global__ void __launch_bounds__(kThreads, SB)
   __syncthreads();
   if (!k.on) return;
   const Scale<VEC> scale(a, k, mean, rstd);
-  const T *const base[1] = {static_cast<const T *>(a.x) + k.n * a.sxn + k.channel()};
-  const int64_t stride[1] = {a.sxl};
-  T *y = static_cast<T *>(a.y) + k.n * a.syn + k.channel();
-  each_position<4, T, VEC, 1>(k, base, stride,
-                              [&](int64_t l, int, Raw<T, VEC>(&raw)[4][1], int count) {
+  Run<T> x[1] = {Run<T>(a.x, k, a.sxn, a.sxl)}, y(a.y, k, a.syn, a.syl);
+  each_position<4, T, VEC, 1>(k, x, [&](Raw<T, VEC>(&raw)[4][1], int count, auto reload) {
+    Vec<VEC> v[4];
 #pragma unroll
-                                for (int u = 0; u < 4; ++u) {
-                                  if (u >= count) break;
-                                  scale.write(raw[u][0], a.act,
-                                              y + (l + (int64_t)u * k.rows) * a.syl);
-                                }
-                              });
+    for (int u = 0; u < 4; ++u) v[u] = values<T, VEC>(raw[u][0]);
+    reload();
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if (u >= count) break;
+      scale.write(v[u], a.act, y.p);
+      y.next();
+    }
+  });
 }
 
 // xh = (x - mu) rstd and dz = dy act'(gamma xh + beta) of a position
@@ -332,13 +353,12 @@ struct Slope {
     ga = params<VEC>(a.gamma, k.channel(), 1.0f, a.wide);
     be = params<VEC>(a.beta, k.channel(), 0.0f, a.wide);
   }
-  template <typename T>
-  __device__ __forceinline__ Vec<VEC> dz(const Raw<T, VEC> &x, const Raw<T, VEC> &dy, int act,
+  __device__ __forceinline__ Vec<VEC> dz(const Vec<VEC> &x, const Vec<VEC> &dy, int act,
                                          Vec<VEC> &xh) const {
-    xh = mul(add(values<T, VEC>(x), mu), rs);
+    xh = mul(add(x, mu), rs);
     Vec<VEC> z = fma(xh, ga, be);
     act_slopes<VEC>(z, act);
-    return mul(values<T, VEC>(dy), z);
+    return mul(dy, z);
   }
 };
 
@@ -358,28 +378,27 @@ __device__ __forceinline__ void grad_sums(const NormArgs &a, const Patch<VEC> &k
 
 // Gradient, first pass: grad_sums, the groups' into means[n][group][piece].
 template <typename T, int VEC>
-__global__ void __launch_bounds__(kThreads, SB)
+__global__ void __launch_bounds__(kThreads, (sample_blocks<VEC, true>()))
     norm_grad_sums_kernel(const __grid_constant__ NormArgs a) {
   __shared__ Sums<T, VEC> buf, s1, s2;
   const Patch<VEC> k(a);
   Vec<VEC> dg = all<VEC>(0.0f), db = dg;
   const Slope<VEC> slope(a, k);
-  if (k.on) {
-    const T *const base[2] = {static_cast<const T *>(a.x) + k.n * a.sxn + k.channel(),
-                              static_cast<const T *>(a.dy) + k.n * a.syn + k.channel()};
-    const int64_t stride[2] = {a.sxl, a.syl};
-    each_position<2, T, VEC, 2>(k, base, stride,
-                                [&](int64_t, int, Raw<T, VEC>(&raw)[2][2], int count) {
+  Run<T> xs[2] = {Run<T>(a.x, k, a.sxn, a.sxl), Run<T>(a.dy, k, a.syn, a.syl)};
+  each_position<2, T, VEC, 2>(k, xs, [&](Raw<T, VEC>(&raw)[2][2], int count, auto reload) {
+    Vec<VEC> x[2], d[2];
 #pragma unroll
-                                  for (int u = 0; u < 2; ++u) {
-                                    if (u >= count) break;
-                                    Vec<VEC> xh;
-                                    const Vec<VEC> dz = slope.template dz<T>(raw[u][0], raw[u][1], a.act, xh);
-                                    db = add(db, dz);
-                                    dg = fma(dz, xh, dg);
-                                  }
-                                });
-  }
+    for (int u = 0; u < 2; ++u) x[u] = values<T, VEC>(raw[u][0]), d[u] = values<T, VEC>(raw[u][1]);
+    reload();
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      if (u >= count) break;
+      Vec<VEC> xh;
+      const Vec<VEC> dz = slope.dz(x[u], d[u], a.act, xh);
+      db = add(db, dz);
+      dg = fma(dz, xh, dg);
+    }
+  });
   grad_sums(a, k, dg, db, slope.ga, buf, s1, s2);
   const int pieces = a.stretches * a.parts, piece = blockIdx.x * a.parts + k.part;
   for (int g = threadIdx.x; g < k.groups; g += kThreads)
@@ -389,17 +408,17 @@ __global__ void __launch_bounds__(kThreads, SB)
 // dx = rstd (gamma dz - m1 - xh m2) of a position; m1 and m2 come times rstd
 template <int VEC, typename T>
 __device__ __forceinline__ void write_dx(const Slope<VEC> &slope, const Vec<VEC> &m1,
-                                         const Vec<VEC> &m2, const Raw<T, VEC> &x,
-                                         const Raw<T, VEC> &dy, int act, T *dx) {
+                                         const Vec<VEC> &m2, const Vec<VEC> &x,
+                                         const Vec<VEC> &dy, int act, T *dx) {
   Vec<VEC> xh;
-  const Vec<VEC> dz = slope.template dz<T>(x, dy, act, xh);
+  const Vec<VEC> dz = slope.dz(x, dy, act, xh);
   const Vec<VEC> o = fma(mul(dz, slope.ga), slope.rs, mul(fma(xh, m2, m1), -1.0f));
   store_vec<T, VEC>(dx, o.v);
 }
 
 // Gradient, second pass: dx.
 template <typename T, int VEC>
-__global__ void __launch_bounds__(kThreads, SB)
+__global__ void __launch_bounds__(kThreads, (sample_blocks<VEC, true>()))
     norm_grad_apply_kernel(const __grid_constant__ NormArgs a) {
   __shared__ Sums<T, VEC> s1, s2;
   const Patch<VEC> k(a);
@@ -415,19 +434,20 @@ __global__ void __launch_bounds__(kThreads, SB)
   const float inv = 1.0f / ((float)a.L * (float)a.w);
   const Vec<VEC> m1 = mul(mul(k.of_groups(s1), inv), slope.rs);
   const Vec<VEC> m2 = mul(mul(k.of_groups(s2), inv), slope.rs);
-  const T *const base[2] = {static_cast<const T *>(a.x) + k.n * a.sxn + k.channel(),
-                            static_cast<const T *>(a.dy) + k.n * a.syn + k.channel()};
-  const int64_t stride[2] = {a.sxl, a.syl};
-  T *dx = static_cast<T *>(a.dx) + k.n * a.sdn + k.channel();
-  each_position<2, T, VEC, 2>(k, base, stride,
-                              [&](int64_t l, int, Raw<T, VEC>(&raw)[2][2], int count) {
+  Run<T> xs[2] = {Run<T>(a.x, k, a.sxn, a.sxl), Run<T>(a.dy, k, a.syn, a.syl)};
+  Run<T> dx(a.dx, k, a.sdn, a.sdl);
+  each_position<2, T, VEC, 2>(k, xs, [&](Raw<T, VEC>(&raw)[2][2], int count, auto reload) {
+    Vec<VEC> x[2], d[2];
 #pragma unroll
-                                for (int u = 0; u < 2; ++u) {
-                                  if (u >= count) break;
-                                  write_dx(slope, m1, m2, raw[u][0], raw[u][1], a.act,
-                                           dx + (l + (int64_t)u * k.rows) * a.sdl);
-                                }
-                              });
+    for (int u = 0; u < 2; ++u) x[u] = values<T, VEC>(raw[u][0]), d[u] = values<T, VEC>(raw[u][1]);
+    reload();
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      if (u >= count) break;
+      write_dx(slope, m1, m2, x[u], d[u], a.act, dx.p);
+      dx.next();
+    }
+  });
 }
 
 // ------------------------------------------------ samples held by a block
@@ -435,23 +455,20 @@ __global__ void __launch_bounds__(kThreads, SB)
 // The block keeps what it read in shared memory; a thread reads back only its
 // own.
 template <typename T, int VEC>
-__global__ void __launch_bounds__(kThreads, SB)
+__global__ void __launch_bounds__(kThreads, (sample_blocks<VEC, false>()))
     norm_block_kernel(const __grid_constant__ NormArgs a) {
   __shared__ Sums<T, VEC> buf, mu, m2;
   const Patch<VEC> k(a);
   Raw<T, VEC> *kept = reinterpret_cast<Raw<T, VEC> *>(norm_smem) + threadIdx.x;
   Spread<VEC> t;
-  if (k.on) {
-    const T *const base[1] = {static_cast<const T *>(a.x) + k.n * a.sxn + k.channel()};
-    const int64_t stride[1] = {a.sxl};
-    each_position<4, T, VEC, 1>(k, base, stride,
-                                [&](int64_t, int slot, Raw<T, VEC>(&raw)[4][1], int count) {
+  Run<T> x[1] = {Run<T>(a.x, k, a.sxn, a.sxl)};
+  int slot = 0;
+  each_position<4, T, VEC, 1>(k, x, [&](Raw<T, VEC>(&raw)[4][1], int count, auto reload) {
 #pragma unroll
-                                  for (int u = 0; u < 4; ++u)
-                                    if (u < count) kept[(slot + u) * kThreads] = raw[u][0];
-                                  t.template take_batch<T, 4>(raw, count);
-                                });
-  }
+    for (int u = 0; u < 4; ++u)
+      if (u < count) kept[slot++ * kThreads] = raw[u][0];
+    t.template take_turn<T, 4>(raw, count, reload);
+  });
   const float n_el = (float)a.L * (float)a.w;
   block_spread(k, t, n_el, buf, mu, m2);
   for (int g = threadIdx.x; g < k.groups; g += kThreads) {
@@ -463,48 +480,50 @@ __global__ void __launch_bounds__(kThreads, SB)
   __syncthreads();
   if (!k.on) return;
   const Scale<VEC> scale(a, k, mu, m2);
-  T *y = static_cast<T *>(a.y) + k.n * a.syn + k.channel();
-  int slot = 0;
-  for (int64_t l = k.row; l < a.L; l += k.rows, ++slot)
-    scale.write(kept[slot * kThreads], a.act, y + l * a.syl);
+  Run<T> y(a.y, k, a.syn, a.syl);
+  for (int i = 0; i < slot; ++i, y.next())
+    scale.write(values<T, VEC>(kept[i * kThreads]), a.act, y.p);
 }
 
 template <typename T, int VEC>
-__global__ void __launch_bounds__(kThreads, SB)
+__global__ void __launch_bounds__(kThreads, (sample_blocks<VEC, true>()))
     norm_block_grad_kernel(const __grid_constant__ NormArgs a) {
   __shared__ Sums<T, VEC> buf, s1, s2;
   const Patch<VEC> k(a);
   Raw<T, VEC> *kept = reinterpret_cast<Raw<T, VEC> *>(norm_smem) + threadIdx.x;
   Vec<VEC> dg = all<VEC>(0.0f), db = dg;
   const Slope<VEC> slope(a, k);
-  if (k.on) {
-    const T *const base[2] = {static_cast<const T *>(a.x) + k.n * a.sxn + k.channel(),
-                              static_cast<const T *>(a.dy) + k.n * a.syn + k.channel()};
-    const int64_t stride[2] = {a.sxl, a.syl};
-    each_position<2, T, VEC, 2>(
-        k, base, stride, [&](int64_t, int slot, Raw<T, VEC>(&raw)[2][2], int count) {
+  Run<T> xs[2] = {Run<T>(a.x, k, a.sxn, a.sxl), Run<T>(a.dy, k, a.syn, a.syl)};
+  int slot = 0;
+  each_position<2, T, VEC, 2>(k, xs, [&](Raw<T, VEC>(&raw)[2][2], int count, auto reload) {
+    Vec<VEC> x[2], d[2];
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            if (u >= count) break;
-            kept[(2 * (slot + u)) * kThreads] = raw[u][0];
-            kept[(2 * (slot + u) + 1) * kThreads] = raw[u][1];
-            Vec<VEC> xh;
-            const Vec<VEC> dz = slope.template dz<T>(raw[u][0], raw[u][1], a.act, xh);
-            db = add(db, dz);
-            dg = fma(dz, xh, dg);
-          }
-        });
-  }
+    for (int u = 0; u < 2; ++u) {
+      x[u] = values<T, VEC>(raw[u][0]), d[u] = values<T, VEC>(raw[u][1]);
+      if (u < count) {
+        kept[2 * slot * kThreads] = raw[u][0];
+        kept[(2 * slot++ + 1) * kThreads] = raw[u][1];
+      }
+    }
+    reload();
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      if (u >= count) break;
+      Vec<VEC> xh;
+      const Vec<VEC> dz = slope.dz(x[u], d[u], a.act, xh);
+      db = add(db, dz);
+      dg = fma(dz, xh, dg);
+    }
+  });
   grad_sums(a, k, dg, db, slope.ga, buf, s1, s2);
   if (!k.on) return;
   const float inv = 1.0f / ((float)a.L * (float)a.w);
   const Vec<VEC> m1 = mul(mul(k.of_groups(s1), inv), slope.rs);
   const Vec<VEC> m2 = mul(mul(k.of_groups(s2), inv), slope.rs);
-  T *dx = static_cast<T *>(a.dx) + k.n * a.sdn + k.channel();
-  int slot = 0;
-  for (int64_t l = k.row; l < a.L; l += k.rows, ++slot)
-    write_dx(slope, m1, m2, kept[(2 * slot) * kThreads], kept[(2 * slot + 1) * kThreads], a.act,
-             dx + l * a.sdl);
+  Run<T> dx(a.dx, k, a.sdn, a.sdl);
+  for (int i = 0; i < slot; ++i, dx.next())
+    write_dx(slope, m1, m2, values<T, VEC>(kept[2 * i * kThreads]),
+             values<T, VEC>(kept[(2 * i + 1) * kThreads]), a.act, dx.p);
 }
 
 }  // namespace
