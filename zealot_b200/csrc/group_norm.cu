@@ -52,7 +52,6 @@ struct NormShape {
   int es;
   bool grad;
   int64_t align;       // bytes that pointers and strides are multiples of: 16, 8, 4 or es
-  int64_t row_stride;  // the largest
 };
 
 // How a call is laid out.
@@ -91,7 +90,7 @@ bool plan_lanes(const NormShape &s, NormPlan *p) {
   // sums, once
   p->blocks = (int)std::max<int64_t>(
       1, std::min<int64_t>((s.N + p->rb - 1) / p->rb, kSms * kLaneBlocks / p->across));
-  return s.row_stride <= INT32_MAX / ((int64_t)p->rb * s.es) && p->across <= 65535;
+  return p->across <= 65535;
 }
 
 // Channels of a block: the whole row where it fits, else as many groups as make
@@ -124,7 +123,7 @@ bool plan_columns(const NormShape &s, int vec, int64_t most_channels, NormPlan *
 NormPlan plan_samples(const NormShape &s) {
   NormPlan p{};
   const int64_t tensors = s.grad ? 2 : 1;
-  for (int vec = std::min(16 / s.es, MAXV); vec >= 1; vec /= 2) {
+  for (int vec = kMaxChannels; vec >= 1; vec /= 2) {
     if (!plan_columns(s, vec, (int64_t)kThreads * vec, &p)) continue;
     // the block form, with columns of 128 bytes or the group if it is wider
     NormPlan b = p;
@@ -147,7 +146,7 @@ NormPlan plan_samples(const NormShape &s) {
     // one wave of the resident blocks, and some positions for each thread
     const int64_t rows = kThreads / (p.cols / vec);
     const int64_t want =
-        std::max<int64_t>(1, kSms * (vec <= 4 ? s.grad ? SGB4 : SB4 : 2) / (p.batch * p.depth));
+        std::max<int64_t>(1, kSms * sample_blocks(s.grad) / (p.batch * p.depth));
     const int64_t fit = std::max<int64_t>(1, s.L / (rows * 4));
     p.stretches = (int)std::max<int64_t>(1, std::min<int64_t>({want, fit, (int64_t)512}));
     p.stretch = ((s.L + p.stretches - 1) / p.stretches + rows * 4 - 1) / (rows * 4) * (rows * 4);
@@ -201,7 +200,6 @@ void use_plan(NormArgs &a, const NormPlan &p, void *workspace) {
   a.part = static_cast<float *>(workspace);
   a.means = reinterpret_cast<float2 *>(a.part + a.N * p.stretches * 2 * a.C);
   a.wide = aligned(a.gamma, 16) && aligned(a.beta, 16);
-  a.one = 1;
 }
 
 zrl_status check_norm(const char *what, int64_t N, int64_t L, int64_t C, int32_t groups,
@@ -230,14 +228,12 @@ void launch_norm(void (*kernel)(NormArgs), dim3 grid, const NormPlan &p, cudaStr
 // What the call's pointers and strides allow.
 NormShape shape_of(const NormArgs &a, int es, bool grad,
                    std::initializer_list<const void *> ptrs) {
-  NormShape s{a.N, a.L, a.C, a.G, es, grad, 16, 1};
+  NormShape s{a.N, a.L, a.C, a.G, es, grad, 16};
   for (const void *p : ptrs)
     while (!aligned(p, s.align)) s.align /= 2;
   for (int64_t t : {a.sxn, a.syn, grad ? a.sdn : a.syn}) {
-    if (a.N > 1) {
+    if (a.N > 1)
       while (t * es % s.align) s.align /= 2;
-      s.row_stride = std::max(s.row_stride, t < 0 ? -t : t);
-    }
   }
   for (int64_t t : {a.sxl, a.syl, grad ? a.sdl : a.syl})
     if (a.L > 1)
@@ -274,11 +270,10 @@ extern "C" int64_t zrl_group_norm_workspace(int64_t N, int64_t L, int64_t C, int
   if (N <= 0 || L <= 0 || C <= 0 || groups < 1 || C % groups) return 0;
   int64_t most = 0;
   for (int es : {2, 4})
-    for (int64_t align = 16; align >= es; align /= 2)
-      for (int64_t row_stride : {(int64_t)1, INT64_MAX}) {
-        const NormShape s{N, L, C, groups, es, grad != 0, align, row_stride};
-        most = std::max(most, workspace_floats(plan_norm(s), s));
-      }
+    for (int64_t align = 16; align >= es; align /= 2) {
+      const NormShape s{N, L, C, groups, es, grad != 0, align};
+      most = std::max(most, workspace_floats(plan_norm(s), s));
+    }
   return most * (int64_t)sizeof(float);
 }
 
@@ -336,16 +331,18 @@ extern "C" zrl_status zrl_group_norm(const void *x, const float *gamma, const fl
       });
       return;
     }
-    for (int64_t n0 = 0; n0 < N; n0 += p.batch) {
-      const NormArgs b = samples_from(a, n0, es);
-      const dim3 grid((unsigned)p.stretches, (unsigned)std::min(p.batch, N - n0),
-                      (unsigned)p.depth);
-      if (p.form == NormPlan::kBlock) {
-        launch_norm(norm_block_kernel<T, VEC>, grid, p, st, b);
-        continue;
+    if constexpr (VEC <= kMaxChannels) {
+      for (int64_t n0 = 0; n0 < N; n0 += p.batch) {
+        const NormArgs b = samples_from(a, n0, es);
+        const dim3 grid((unsigned)p.stretches, (unsigned)std::min(p.batch, N - n0),
+                        (unsigned)p.depth);
+        if (p.form == NormPlan::kBlock) {
+          launch_norm(norm_block_kernel<T, VEC>, grid, p, st, b);
+          continue;
+        }
+        norm_stats_kernel<T, VEC><<<grid, kThreads, 0, st>>>(b);
+        norm_apply_kernel<T, VEC><<<grid, kThreads, 0, st>>>(b);
       }
-      norm_stats_kernel<T, VEC><<<grid, kThreads, 0, st>>>(b);
-      norm_apply_kernel<T, VEC><<<grid, kThreads, 0, st>>>(b);
     }
   });
   return seq_launched("group_norm");
@@ -411,16 +408,18 @@ extern "C" zrl_status zrl_group_norm_grad(const void *x, const void *dy, const f
       sums = p.blocks;
       return;
     }
-    for (int64_t n0 = 0; n0 < N; n0 += p.batch) {
-      const NormArgs b = samples_from(a, n0, es);
-      const dim3 grid((unsigned)p.stretches, (unsigned)std::min(p.batch, N - n0),
-                      (unsigned)p.depth);
-      if (p.form == NormPlan::kBlock) {
-        launch_norm(norm_block_grad_kernel<T, VEC>, grid, p, st, b);
-        continue;
+    if constexpr (VEC <= kMaxChannels) {
+      for (int64_t n0 = 0; n0 < N; n0 += p.batch) {
+        const NormArgs b = samples_from(a, n0, es);
+        const dim3 grid((unsigned)p.stretches, (unsigned)std::min(p.batch, N - n0),
+                        (unsigned)p.depth);
+        if (p.form == NormPlan::kBlock) {
+          launch_norm(norm_block_grad_kernel<T, VEC>, grid, p, st, b);
+          continue;
+        }
+        norm_grad_sums_kernel<T, VEC><<<grid, kThreads, 0, st>>>(b);
+        norm_grad_apply_kernel<T, VEC><<<grid, kThreads, 0, st>>>(b);
       }
-      norm_grad_sums_kernel<T, VEC><<<grid, kThreads, 0, st>>>(b);
-      norm_grad_apply_kernel<T, VEC><<<grid, kThreads, 0, st>>>(b);
     }
   });
   launch_column_sum(a.part, sums, 2 * C, ParamOut{dgamma, dbeta, C}, st);

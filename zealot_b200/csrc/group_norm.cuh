@@ -19,8 +19,7 @@ struct NormArgs {
   int64_t N, L, sxn, sxl, syn, syl, sdn, sdl;  // strides of x, y / dy, dx
   int32_t C, G, w, act;
   float eps;
-  bool wide;    // gamma and beta start on 16 bytes
-  int32_t one;  // 1
+  bool wide;  // gamma and beta start on 16 bytes
   // rows: lanes per group, groups of a block, rows of a block
   int32_t p, gb, rb;
   // samples: channels of a block at most, parts of a wide group, stretches of

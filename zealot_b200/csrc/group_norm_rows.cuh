@@ -8,7 +8,9 @@
 namespace zrl {
 namespace {
 
-constexpr int kLaneBlocks = 2;  // resident blocks
+// Resident blocks, which bounds the registers.  Three spill where a lane has four
+// single channels: 98304 x 250 f32 forward 62 -> 109 us.
+constexpr int kLaneBlocks = 2;
 
 // A thread of the row form: E vectors of VEC channels of one group, the same
 // ones in every row it meets, so its gammas and betas stay in registers.
@@ -36,37 +38,6 @@ struct RowLanes {
   }
 };
 
-// p + stride as one multiply-add (one is 1, which the compiler cannot know).
-template <typename P>
-__device__ __forceinline__ void advance(P *&p, int32_t stride, int32_t one) {
-  asm("mad.wide.s32 %0, %1, %2, %0;" : "+l"(p) : "r"(stride), "r"(one));
-}
-
-// A thread's places in one tensor: a running pointer per vector, U steps of rb
-// rows a turn.
-template <typename T, int E>
-struct RowPlaces {
-  T *p[E];
-  int32_t step;  // bytes from a row to the one rb below
-  int64_t jump;  // bytes from the end of a turn to the next
-  __device__ __forceinline__ RowPlaces(const void *base, int64_t stride, const int64_t *at,
-                                       int64_t first, const NormArgs &a, int U) {
-#pragma unroll
-    for (int e = 0; e < E; ++e)
-      p[e] = const_cast<T *>(static_cast<const T *>(base)) + first * stride + at[e];
-    step = (int32_t)(a.rb * stride * (int64_t)sizeof(T));
-    jump = (int64_t)(gridDim.x - 1) * U * step;
-  }
-  __device__ __forceinline__ void next_row(int32_t one) {
-#pragma unroll
-    for (int e = 0; e < E; ++e) advance(p[e], step, one);
-  }
-  __device__ __forceinline__ void next_turn() {
-#pragma unroll
-    for (int e = 0; e < E; ++e) p[e] = (T *)((char *)p[e] + jump);
-  }
-};
-
 // U rows rb apart at a time; the next ones' loads are in flight.
 template <typename T, int VEC, int E>
 __global__ void __launch_bounds__(kThreads, kLaneBlocks)
@@ -76,20 +47,20 @@ __global__ void __launch_bounds__(kThreads, kLaneBlocks)
   const float inv = 1.0f / (float)a.w;
   const int64_t pace = (int64_t)gridDim.x * a.rb * U;
   int64_t n = (int64_t)blockIdx.x * a.rb * U + k.r;  // this thread's first row
-  RowPlaces<T, E> xs(a.x, a.sxn, k.at, n, a, U), ys(a.y, a.syn, k.at, n, a, U);
+  // rows follow by adding strides; a vector's offset is added at each access
+  const T *x0 = static_cast<const T *>(a.x) + n * a.sxn;
+  T *y0 = static_cast<T *>(a.y) + n * a.syn;
+  const int64_t xu = a.rb * a.sxn, yu = a.rb * a.syn;
   Raw<T, VEC> raw[U][E];
   auto load = [&](int64_t first) {
-    const bool whole = first + (U - 1) * a.rb < a.N;
+    const T *xr = x0;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (whole || first + u * a.rb < a.N) {
+    for (int u = 0; u < U; ++u, xr += xu)
 #pragma unroll
-        for (int e = 0; e < E; ++e)
-          if (k.has[e]) raw[u][e] = *reinterpret_cast<const Raw<T, VEC> *>(xs.p[e]);
-      }
-      xs.next_row(a.one);
-    }
-    xs.next_turn();
+      for (int e = 0; e < E; ++e)
+        if (first + u * a.rb < a.N && k.has[e])
+          raw[u][e] = *reinterpret_cast<const Raw<T, VEC> *>(xr + k.at[e]);
+    x0 += pace * a.sxn;
   };
 #pragma unroll
   for (int u = 0; u < U; ++u)
@@ -123,23 +94,22 @@ __global__ void __launch_bounds__(kThreads, kLaneBlocks)
       rstd[u] = sum(q);
     }
     lanes_sum(rstd, a.p);
-    const bool whole = n + (U - 1) * a.rb < a.N;
+    T *yr = y0;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
+    for (int u = 0; u < U; ++u, yr += yu) {
+      const int64_t row = n + u * a.rb;
       const float r = rsqrtf(fmaf(rstd[u], inv, a.eps));
-      if (whole || n + u * a.rb < a.N) {
+      if (row >= a.N) break;
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-          Vec<VEC> z = fma(x[u][e], mul(k.ga[e], r), k.be[e]);
-          act_values<VEC>(z, a.act);
-          if (k.has[e]) store_vec<T, VEC>(ys.p[e], z.v);
-        }
-        if (k.lead && a.mean) a.mean[(n + u * a.rb) * a.G + k.g] = mu[u];
-        if (k.lead && a.rstd) a.rstd[(n + u * a.rb) * a.G + k.g] = r;
+      for (int e = 0; e < E; ++e) {
+        Vec<VEC> z = fma(x[u][e], mul(k.ga[e], r), k.be[e]);
+        act_values<VEC>(z, a.act);
+        if (k.has[e]) store_vec<T, VEC>(yr + k.at[e], z.v);
       }
-      ys.next_row(a.one);
+      if (k.lead && a.mean) a.mean[row * a.G + k.g] = mu[u];
+      if (k.lead && a.rstd) a.rstd[row * a.G + k.g] = r;
     }
-    ys.next_turn();
+    y0 += pace * a.syn;
   }
 }
 
