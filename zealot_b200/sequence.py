@@ -36,11 +36,11 @@ def _invalid(msg: str):
 
 
 def _dtype(x) -> int:
-    if not x.is_cuda:
-        raise TypeError(f"tensor on {x.device}: these operators take CUDA tensors")
     dt = _DTYPES.get(x.dtype)
     if dt is None:
         raise TypeError(f"element type {x.dtype}: float32, bfloat16 or float16")
+    if not x.is_cuda:
+        raise TypeError(f"tensor on {x.device}: these operators take CUDA tensors")
     return dt
 
 
@@ -100,11 +100,10 @@ def _f32(name, t, shape, device):
     """The address of an fp32 parameter, state or statistic; None stays None."""
     if t is None:
         return None
-    if t.dtype != _F32 or t.device != device or t.shape != shape:
-        _same(name, t, shape, _F32, device)
-    if not t.is_contiguous():
-        raise _invalid(f"{name}: not contiguous")
-    return t.data_ptr()
+    if t.dtype is _F32 and t.shape == shape and t.is_contiguous() and t.device == device:
+        return t.data_ptr()
+    _same(name, t, shape, _F32, device)
+    raise _invalid(f"{name}: not contiguous")
 
 
 def _bt(name, t):
@@ -126,8 +125,11 @@ def _like(x):
 
 def _scan_inputs(x, rec, inp, lam, h0, resets, shape, dev):
     """Checks what forward and gradient share; (lam, h0, resets) addresses."""
-    _same("rec", rec, shape, x.dtype, dev)
-    _same("inp", inp, shape, x.dtype, dev)
+    t = x.dtype
+    if not (rec.dtype is t and inp.dtype is t and rec.shape == shape and inp.shape == shape and
+            rec.device == dev and inp.device == dev):
+        _same("rec", rec, shape, t, dev)
+        _same("inp", inp, shape, t, dev)
     D = shape[-1]
     p_z = None
     if resets is not None:
@@ -201,18 +203,22 @@ def gated_step(x, rec, inp, lam, state, resets=None, c: float = 8.0, out=None):
         raise _invalid("state: a float32 tensor [B, D]")
     p_lam, p_h0, p_z = _scan_inputs(x, rec, inp, lam, state, resets, shape, dev)
     B, D = shape
-    h = _dense_like(x)
+    dense = x.is_contiguous()
+    h = torch.empty_like(x) if dense else _dense_like(x)
     if out is None:
         out = torch.empty_like(state)
+        p_out = out.data_ptr()
+    else:
+        p_out = _f32("out", out, shape, dev)
     st = None
-    if not (x.is_contiguous() and rec.is_contiguous() and inp.is_contiguous() and
+    if not (dense and rec.is_contiguous() and inp.is_contiguous() and
             (resets is None or resets.is_contiguous())):
-        if D > 1 and any(t.stride(1) != 1 for t in (x, rec, inp)):
+        if D > 1 and (x.stride(1) != 1 or rec.stride(1) != 1 or inp.stride(1) != 1):
             raise _invalid("x, rec, inp: the last axis is not dense")
         z = resets.stride(0) if resets is not None else 0
         st = (C.c_int64 * 10)(x.stride(0), 0, rec.stride(0), 0, inp.stride(0), 0, z, 0, D, 0)
     _call(N.lib().zrl_gated_scan, dev, x.data_ptr(), rec.data_ptr(), inp.data_ptr(), p_lam,
-          p_h0, p_z, B, 1, D, dt, c, st, h.data_ptr(), _f32("out", out, shape, dev), None, None, 0)
+          p_h0, p_z, B, 1, D, dt, c, st, h.data_ptr(), p_out, None, None, 0)
     return h, out
 
 
