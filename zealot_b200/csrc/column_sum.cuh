@@ -5,6 +5,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "seq_common.cuh"
+
 namespace zrl {
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -40,6 +42,7 @@ __global__ void __launch_bounds__(1024) column_sum_kernel(const float *part, int
   const int lane = threadIdx.x & 31, wy = threadIdx.x >> 5;
   const int64_t d = (int64_t)(blockIdx.x / ranks) * 32 + lane;
   if (ranks > 1) cluster_barrier();  // every block of the cluster runs
+  wait_for_previous();
   float s = 0.0f;
   if (d < cols) {
 #pragma unroll 4
@@ -64,27 +67,13 @@ __global__ void __launch_bounds__(1024) column_sum_kernel(const float *part, int
   if (wy == 0 && rank == 0 && d < cols) out(d, s);
 }
 
-// The launch error, if any, is left for cudaGetLastError.
+// After the kernel that wrote part.
 template <typename Out>
 inline void launch_column_sum(const float *part, int64_t rows, int64_t cols, Out out,
                               cudaStream_t st) {
   const int ranks = rows >= 256 ? 8 : 1;
-  const unsigned blocks = (unsigned)((cols + 31) / 32 * ranks);
-  if (ranks == 1) {
-    column_sum_kernel<<<blocks, 1024, 0, st>>>(part, rows, cols, out);
-    return;
-  }
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(blocks);
-  cfg.blockDim = dim3(1024);
-  cfg.stream = st;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = (unsigned)ranks;
-  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  (void)cudaLaunchKernelEx(&cfg, column_sum_kernel<Out>, part, rows, cols, out);
+  launch_next(column_sum_kernel<Out>, dim3((unsigned)((cols + 31) / 32 * ranks)), dim3(1024),
+              ranks, st, part, rows, cols, out);
 }
 
 }  // namespace zrl

@@ -309,6 +309,7 @@ __global__ void __launch_bounds__(256, resident<T>()) scan_fold_kernel(const __g
     else
       run(std::false_type{}, std::false_type{});
   }
+  let_next_start();
 #pragma unroll
   for (int v = 0; v < V; ++v) agg[wt][v * 32 + lane] = make_float2(P[v], H[v]);
   __syncthreads();
@@ -337,6 +338,7 @@ template <bool BACK, int V>
 __device__ __forceinline__ void enter_slab(const ScanArgs &a, const Slab &slab, const Place<V> &at,
                                            Vec<V> &h) {
   if (a.slabs == 1) return;
+  wait_for_previous();
   const int64_t c = at.b * a.D + at.d, row = a.B * a.D;
   const int blocks = gridDim.y, mine = blockIdx.y;
 #pragma unroll 8
@@ -561,6 +563,7 @@ __global__ void __launch_bounds__(256, kGradResident)
     else finish(std::false_type{});
     load_fwd(t0, n);
   }
+  let_next_start();
   if (at.live && slab.index < a.slabs) {
 #pragma unroll
     for (int v = 0; v < V; ++v) {
@@ -811,7 +814,8 @@ extern "C" zrl_status zrl_gated_scan(const void *x, const void *rec, const void 
       return;
     }
     if (p.slabs > 1) scan_fold_kernel<E, V, false><<<grid, threads, 0, st>>>(a);
-    scan_kernel<E, V><<<grid, threads, 0, st>>>(a);
+    if (p.slabs > 1) launch_next(scan_kernel<E, V>, grid, threads, 1, st, a);
+    else scan_kernel<E, V><<<grid, threads, 0, st>>>(a);
   });
   return seq_launched("gated_scan");
 }
@@ -878,7 +882,8 @@ extern "C" zrl_status zrl_gated_scan_grad(
       constexpr int V = decltype(v)::value;
       const dim3 grid((unsigned)p.blocks, (unsigned)p.slab_blocks), threads(32, kWarps);
       if (p.slabs > 1) scan_fold_kernel<E, V, true><<<grid, threads, 0, st>>>(a);
-      scan_grad_kernel<E, V><<<grid, threads, 0, st>>>(a);
+      if (p.slabs > 1) launch_next(scan_grad_kernel<E, V>, grid, threads, 1, st, a);
+      else scan_grad_kernel<E, V><<<grid, threads, 0, st>>>(a);
     });
   launch_column_sum(a.part, B * p.slabs, D, DlamOut{lam, dlam, c}, st);
   return seq_launched("gated_scan_grad");

@@ -341,7 +341,7 @@ extern "C" zrl_status zrl_group_norm(const void *x, const float *gamma, const fl
           continue;
         }
         norm_stats_kernel<T, VEC><<<grid, kThreads, 0, st>>>(b);
-        norm_apply_kernel<T, VEC><<<grid, kThreads, 0, st>>>(b);
+        launch_next(norm_apply_kernel<T, VEC>, grid, dim3(kThreads), 1, st, b);
       }
     }
   });
@@ -418,7 +418,7 @@ extern "C" zrl_status zrl_group_norm_grad(const void *x, const void *dy, const f
           continue;
         }
         norm_grad_sums_kernel<T, VEC><<<grid, kThreads, 0, st>>>(b);
-        norm_grad_apply_kernel<T, VEC><<<grid, kThreads, 0, st>>>(b);
+        launch_next(norm_grad_apply_kernel<T, VEC>, grid, dim3(kThreads), 1, st, b);
       }
     }
   });

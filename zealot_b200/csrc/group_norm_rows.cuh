@@ -202,6 +202,7 @@ __global__ void __launch_bounds__(kThreads, kLaneBlocks)
     }
     o0 += pace * a.sdn;
   }
+  let_next_start();
   // the rows of the block, in order
   const int per_row = a.gb * a.p;
 #pragma unroll

@@ -255,6 +255,7 @@ __global__ void __launch_bounds__(kThreads, sample_blocks(false))
   each_position<4, T, VEC, 1>(k, x, [&](Raw<T, VEC>(&raw)[4][1], int count, auto reload) {
     t.template take_turn<T, 4>(raw, count, reload);
   });
+  let_next_start();
   block_spread(k, t, (float)(k.l1 - k.l0) * (float)k.per, buf, mu, m2);
   const int pieces = a.stretches * a.parts, piece = blockIdx.x * a.parts + k.part;
   float2 *p = reinterpret_cast<float2 *>(a.part);
@@ -295,6 +296,7 @@ __global__ void __launch_bounds__(kThreads, sample_blocks(false))
     return (float)(min(a.L, l0 + a.stretch) - l0) *
            (float)(a.parts == 1 ? a.w : min(a.cols, a.w - c0));
   };
+  wait_for_previous();
   pieces_sums(k, pieces, [&](int g, int i) { return count(i) * p[g * pieces + i].x; },
               [&](int g, float s) { mean[g] = s * inv; });
   __syncthreads();
@@ -392,6 +394,7 @@ __global__ void __launch_bounds__(kThreads, sample_blocks(true))
       dg = fma(dz, xh, dg);
     }
   });
+  let_next_start();
   grad_sums(a, k, dg, db, slope.ga, buf, s1, s2);
   const int pieces = a.stretches * a.parts, piece = blockIdx.x * a.parts + k.part;
   for (int g = threadIdx.x; g < k.groups; g += kThreads)
@@ -417,6 +420,7 @@ __global__ void __launch_bounds__(kThreads, sample_blocks(true))
   const Patch<VEC> k(a);
   const int pieces = a.stretches * a.parts;
   const float2 *p = a.means + (k.n * a.G + k.g0) * pieces;
+  wait_for_previous();
   pieces_sums(k, pieces, [&](int g, int i) { return p[g * pieces + i].x; },
               [&](int g, float s) { s1[g] = s; });
   pieces_sums(k, pieces, [&](int g, int i) { return p[g * pieces + i].y; },
@@ -441,6 +445,7 @@ __global__ void __launch_bounds__(kThreads, sample_blocks(true))
       dx.next();
     }
   });
+  let_next_start();
 }
 
 // ------------------------------------------------ samples held by a block
@@ -508,6 +513,7 @@ __global__ void __launch_bounds__(kThreads, sample_blocks(true))
       dg = fma(dz, xh, dg);
     }
   });
+  let_next_start();
   grad_sums(a, k, dg, db, slope.ga, buf, s1, s2);
   if (!k.on) return;
   const float inv = 1.0f / ((float)a.L * (float)a.w);

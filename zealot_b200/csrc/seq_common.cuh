@@ -221,6 +221,34 @@ __device__ __forceinline__ void store_vec(T *p, const float *in) {
   *reinterpret_cast<Raw<T, V> *>(p) = pack<T, V>(in);
 }
 
+// A kernel that reads what the kernel before it wrote is launched to start while
+// that one ends (launch_next): it waits here before it reads or writes any of
+// that, and the earlier kernel says near its end that blocks may start.
+__device__ __forceinline__ void wait_for_previous() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+__device__ __forceinline__ void let_next_start() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+// The launch error, if any, is left for cudaGetLastError.
+template <typename... P, typename... A>
+inline void launch_next(void (*kernel)(P...), dim3 grid, dim3 block, int cluster,
+                        cudaStream_t st, A... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.stream = st;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = (unsigned)cluster;
+  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  (void)cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 // Calls f with a value of the element type that dtype names.
 template <typename F>
 inline void with_dtype(int32_t dtype, F &&f) {
