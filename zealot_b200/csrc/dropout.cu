@@ -18,7 +18,7 @@ struct DropoutArgs {
   void *y;
   int64_t sx, sr, sy;  // row strides, elements
   int64_t N, row0;     // rows of this launch, number of the first (rows == NULL)
-  int32_t D, groups;   // columns; groups of 8 columns, or segments of 256
+  int32_t D, groups;   // columns; groups of 8 columns, or segments
   uint32_t drop;       // a lane below this is dropped
   float scale;
   uint2 key;
@@ -89,36 +89,43 @@ __global__ void __launch_bounds__(256) dropout_vec_kernel(const __grid_constant_
   }
 }
 
-// Any width, stride and alignment: a warp per row and segment of 256 columns.
-// Lane l draws group l; column k * 32 + l of the segment takes its bit from the
-// lane that has its group, so every access is to 32 neighbouring elements.
-// 98304 x 333 f32: 55 us (4.8 TB/s); a thread per group took 146.
-template <typename T>
+// Any width, stride and alignment: W = 2^WIDE lanes per row and segment of 8 W
+// columns.  Lane l of them draws group l; column k W + l takes its bit from
+// the lane that has its group, so every access is to neighbouring elements.
+// 98304 x 333 f32: 51 us (5.1 TB/s); a thread per group took 146.
+template <typename T, int WIDE>
 __global__ void __launch_bounds__(256) dropout_kernel(const __grid_constant__ DropoutArgs a) {
-  const uint32_t lane = threadIdx.x & 31, total = (uint32_t)(a.N * a.groups);
-  for (uint32_t e = blockIdx.x * 8 + (threadIdx.x >> 5); e < total; e += gridDim.x * 8) {
-    const uint32_t row = quotient(a, e), segment = e - row * a.groups;
+  constexpr uint32_t W = 1u << WIDE, at_once = 32u >> WIDE;
+  const uint32_t lane = threadIdx.x & 31, q = lane & (W - 1);
+  const uint32_t total = (uint32_t)(a.N * a.groups);
+  // every lane of a warp takes part in the exchange, with a row or without
+  for (uint32_t e0 = (blockIdx.x * 8 + (threadIdx.x >> 5)) * at_once; e0 < total;
+       e0 += gridDim.x * 8 * at_once) {
+    const uint32_t e = e0 + (lane >> WIDE);
+    const bool on = e < total;
+    const uint32_t row = on ? quotient(a, e) : 0, segment = on ? e - row * a.groups : 0;
     const int64_t id = a.rows ? a.rows[row] : a.row0 + row;
-    const int c0 = segment * 256 + lane;
+    const int c0 = segment * 8 * W + q, end = on ? a.D : 0;
     const T *x = static_cast<const T *>(a.x) + (int64_t)row * a.sx + c0;
     const T *r = static_cast<const T *>(a.residual) + (int64_t)row * a.sr + c0;
     T *y = static_cast<T *>(a.y) + (int64_t)row * a.sy + c0;
     T xv[8], rv[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      if (c0 + k * 32 < a.D) {
-        xv[k] = x[k * 32];
-        if (a.residual) rv[k] = r[k * 32];
+      if (c0 + (k << WIDE) < end) {
+        xv[k] = x[k << WIDE];
+        if (a.residual) rv[k] = r[k << WIDE];
       }
     }
-    const uint32_t mine = keep_bits(a, id, segment * 32 + lane);
+    const uint32_t mine = keep_bits(a, id, segment * W + q);
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      const uint32_t bits = __shfl_sync(0xffffffffu, mine, k * 4 + (lane >> 3));
-      if (c0 + k * 32 < a.D) {
-        float v = bits >> (lane & 7) & 1 ? to_f32(xv[k]) * a.scale : 0.0f;
+      const uint32_t c = (k << WIDE) + q;  // of the segment
+      const uint32_t bits = __shfl_sync(0xffffffffu, mine, (lane - q) + (c >> 3));
+      if (c0 + (k << WIDE) < end) {
+        float v = bits >> (c & 7) & 1 ? to_f32(xv[k]) * a.scale : 0.0f;
         if (a.residual) v += to_f32(rv[k]);
-        y[k * 32] = from_f32<T>(v);
+        y[k << WIDE] = from_f32<T>(v);
       }
     }
   }
@@ -160,7 +167,14 @@ extern "C" zrl_status zrl_dropout(const void *x, const void *residual, const int
   a.stream_id = stream_id;
   bool vec = D % 8 == 0 && aligned(x, 16) && aligned(y, 16) && aligned(residual, 16);
   for (int64_t st : {a.sx, residual ? a.sr : a.sx, a.sy}) vec = vec && (N == 1 || st * es % 16 == 0);
-  a.groups = (int32_t)(vec ? D / 8 : (D + 255) / 256);
+  // the segment that leaves the fewest lanes without columns, the widest of them
+  int wide = 5;
+  int64_t best = INT64_MAX;
+  for (int w : {5, 4, 3, 1}) {
+    const int64_t lanes = (D + (8 << w) - 1) / (8 << w) << w;
+    if (lanes < best && (w >= 3 || D <= 8 << w)) best = lanes, wide = w;
+  }
+  a.groups = (int32_t)(vec ? D / 8 : (D + (8 << wide) - 1) / (8 << wide));
   while ((1u << a.shift) < (uint32_t)a.groups) ++a.shift;
   a.shift = a.shift ? a.shift - 1 : 0;
   a.magic = (uint32_t)((((uint64_t)1 << (32 + a.shift)) + a.groups - 1) / a.groups);
@@ -170,11 +184,14 @@ extern "C" zrl_status zrl_dropout(const void *x, const void *residual, const int
   for (int64_t n0 = 0; n0 < N; n0 += most) {
     a.N = std::min(most, N - n0);
     a.row0 = n0;
-    const int64_t units = vec ? (a.N * a.groups + 255) / 256 : (a.N * a.groups + 7) / 8;
+    const int64_t units = vec ? (a.N * a.groups + 255) / 256 : ((a.N * a.groups << wide) + 255) / 256;
     const unsigned blocks = (unsigned)std::min<int64_t>(units, 148 * (vec ? 4 : 16));
     with_dtype(dtype, [&](auto t) {
       using T = decltype(t);
-      if (!vec) dropout_kernel<T><<<blocks, 256, 0, st>>>(a);
+      if (!vec && wide == 5) dropout_kernel<T, 5><<<blocks, 256, 0, st>>>(a);
+      else if (!vec && wide == 4) dropout_kernel<T, 4><<<blocks, 256, 0, st>>>(a);
+      else if (!vec && wide == 3) dropout_kernel<T, 3><<<blocks, 256, 0, st>>>(a);
+      else if (!vec) dropout_kernel<T, 1><<<blocks, 256, 0, st>>>(a);
       else if (residual) dropout_vec_kernel<T, true><<<blocks, 256, 0, st>>>(a);
       else dropout_vec_kernel<T, false><<<blocks, 256, 0, st>>>(a);
     });

@@ -21,7 +21,7 @@ namespace {
 
 constexpr int kSteps = 8;       // steps of a stretch
 constexpr int kWarps = 8;       // warps of a block at most
-constexpr int kMinSlab = 32;    // steps of a slab at least
+constexpr int kMinSlab = 16;    // steps of a slab at least
 // The forward call keeps the state before every stretch after the first; the
 // gradient recomputes the states inside a stretch from there.
 constexpr int kChunk = kSteps;
@@ -32,6 +32,7 @@ constexpr float kTinySquare = 7.5231638e-37f;  // 2^-120
 // (device us, 2 / 3 / 4 blocks): forward 1024 x 24 x 512 bf16 35 / 34 / 32, 4096 x
 // 24 x 128 f32 41 / 47 / 55 (spills); gradient of the former 49 / 110 / - (spills).
 template <typename T> constexpr int resident() { return sizeof(T) == 2 ? 4 : 2; }
+// (f32's gradient takes one channel a lane: pairs spill, 78 against 106 us.)
 constexpr int kGradResident = 2;
 
 struct ScanArgs {
@@ -639,10 +640,11 @@ struct DlamOut {
 // where rows and channels fill the SMs (kFull groups of lanes) or the row is
 // short; else the row is cut into slabs, whose effect on the state is folded in
 // a first pass: as many blocks of eight slabs as fill one to three waves of the
-// resident blocks best.  Measured (fold + scan, device us): 1 x 65536 x 512 f32 in
-// 1 / 1.5 / 3 waves 152 / 171 / 169.
+// resident blocks best.  Measured (device us): 1 x 65536 x 512 f32 fold + scan in 1
+// / 1.5 / 3 waves 152 / 171 / 169; 200 x 400 x 480 bf16 with gradient (1,500 groups) in
+// one piece 315, in slabs 369; 16 x 100 x 200 f16 (50 groups) 65 and 38.
 constexpr int kSms = 148;
-constexpr int64_t kFull = kSms * 16;
+constexpr int64_t kFull = kSms * 8;
 struct ScanPlan {
   int V, slabs, slab_blocks;
   int64_t units, slab_steps, blocks;
@@ -870,7 +872,8 @@ extern "C" zrl_status zrl_gated_scan_grad(
   bool pairs = false;
   if (!place_tensors(ts, 7, strides, T, D, es, &pairs))
     return seq_fail(ZRL_NOT_SUPPORTED, "gated_scan_grad: a time stride of 2 GiB or more");
-  const ScanPlan p = plan_scan(B, T, D, pairs ? 2 : 1, kGradResident);
+  const int V = pairs && es == 2 ? 2 : 1;
+  const ScanPlan p = plan_scan(B, T, D, V, kGradResident);
   if (p.blocks > 0x7fffffff)
     return seq_fail(ZRL_NOT_SUPPORTED, "gated_scan_grad: B * D too large");
   use_plan(a, p, workspace);
@@ -880,10 +883,12 @@ extern "C" zrl_status zrl_gated_scan_grad(
     with_plan(dtype, p, [&](auto t, auto v) {
       using E = decltype(t);
       constexpr int V = decltype(v)::value;
-      const dim3 grid((unsigned)p.blocks, (unsigned)p.slab_blocks), threads(32, kWarps);
-      if (p.slabs > 1) scan_fold_kernel<E, V, true><<<grid, threads, 0, st>>>(a);
-      if (p.slabs > 1) launch_next(scan_grad_kernel<E, V>, grid, threads, 1, st, a);
-      else scan_grad_kernel<E, V><<<grid, threads, 0, st>>>(a);
+      if constexpr (V * sizeof(E) <= 4) {
+        const dim3 grid((unsigned)p.blocks, (unsigned)p.slab_blocks), threads(32, kWarps);
+        if (p.slabs > 1) scan_fold_kernel<E, V, true><<<grid, threads, 0, st>>>(a);
+        if (p.slabs > 1) launch_next(scan_grad_kernel<E, V>, grid, threads, 1, st, a);
+        else scan_grad_kernel<E, V><<<grid, threads, 0, st>>>(a);
+      }
     });
   launch_column_sum(a.part, B * p.slabs, D, DlamOut{lam, dlam, c}, st);
   return seq_launched("gated_scan_grad");

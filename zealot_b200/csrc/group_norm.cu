@@ -75,8 +75,8 @@ bool plan_lanes(const NormShape &s, NormPlan *p) {
   while (w % vec || s.align % (vec * s.es)) vec /= 2;
   const int64_t nv = w / vec, most = vec >= 4 ? 2 : 4;
   int64_t E = 1;
-  while (E < most && E * vec < 8 && 8 * E < nv) E *= 2;
-  while (E < most && (nv + E - 1) / E > 32) E *= 2;
+  while (E < most && E * vec < 8 && 8 * E < nv) ++E;
+  while (E < most && (nv + E - 1) / E > 32) ++E;
   if ((nv + E - 1) / E > 32) return false;
   p->form = NormPlan::kLanes;
   p->vec = vec;
@@ -186,7 +186,10 @@ template <int VEC, typename F>
 void with_e(int E, F &&f) {
   if (E == 1) f(std::integral_constant<int, 1>{});
   else if (E == 2) f(std::integral_constant<int, 2>{});
-  else if constexpr (VEC <= 2) f(std::integral_constant<int, 4>{});
+  else if constexpr (VEC <= 2) {
+    if (E == 3) f(std::integral_constant<int, 3>{});
+    else f(std::integral_constant<int, 4>{});
+  }
 }
 
 void use_plan(NormArgs &a, const NormPlan &p, void *workspace) {
