@@ -38,7 +38,11 @@ struct RowLanes {
   }
 };
 
-// U rows rb apart at a time; the next ones' loads are in flight.
+// U rows rb apart at a time; the next ones' loads are in flight.  Bound by issue
+// slots at the sixteen warps an SM that its registers allow: 24576 x 512 bf16 in
+// groups of 32 ELU 12 us (4.2 TB/s), 98304 x 250 f32 in groups of 25 SiLU 62 us (3.2
+// TB/s: single channels, 55 slots each; rows staged as flat tiles in shared memory
+// took 70).
 template <typename T, int VEC, int E>
 __global__ void __launch_bounds__(kThreads, kLaneBlocks)
     norm_rows_kernel(const __grid_constant__ NormArgs a) {
@@ -114,7 +118,7 @@ __global__ void __launch_bounds__(kThreads, kLaneBlocks)
 }
 
 // dx, and part[block][2][C]: the block's sums for dgamma and dbeta, kept in
-// registers over all its rows.
+// registers over all its rows.  98304 x 250 f32 in groups of 25 SiLU 101 us (2.9 TB/s).
 template <typename T, int VEC, int E>
 __global__ void __launch_bounds__(kThreads, kLaneBlocks)
     norm_rows_grad_kernel(const __grid_constant__ NormArgs a) {

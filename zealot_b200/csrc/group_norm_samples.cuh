@@ -244,7 +244,8 @@ __device__ __forceinline__ void block_spread(const Patch<VEC> &k, const Spread<V
 }
 
 // First pass: part[n][group][piece] = (mean, squares about it) of the block's
-// piece.
+// piece.  64 x 5046 x 64 f16 14 us (2.9 TB/s): a block lives for 15 turns, its ramp and
+// its sums are a third of that.
 template <typename T, int VEC>
 __global__ void __launch_bounds__(kThreads, sample_blocks(false))
     norm_stats_kernel(const __grid_constant__ NormArgs a) {
@@ -281,7 +282,8 @@ struct Scale {
   }
 };
 
-// Second pass: the pieces' means and squares give the group's, then y.
+// Second pass: the pieces' means and squares give the group's, then y.  64 x 5046 x
+// 64 f16 ELU 14 us, 16 x 6360 x 256 bf16 GELU 31 us (26 issue slots a value).
 template <typename T, int VEC>
 __global__ void __launch_bounds__(kThreads, sample_blocks(false))
     norm_apply_kernel(const __grid_constant__ NormArgs a) {
@@ -371,7 +373,8 @@ __device__ __forceinline__ void grad_sums(const NormArgs &a, const Patch<VEC> &k
   group_sums(k, mul(dg, ga), buf, s2);
 }
 
-// Gradient, first pass: grad_sums, the groups' into means[n][group][piece].
+// Gradient, first pass: grad_sums, the groups' into means[n][group][piece].  16 x
+// 6360 x 256 bf16 GELU 35 us (3.0 TB/s); 26 issue slots a value.
 template <typename T, int VEC>
 __global__ void __launch_bounds__(kThreads, sample_blocks(true))
     norm_grad_sums_kernel(const __grid_constant__ NormArgs a) {
@@ -412,7 +415,7 @@ __device__ __forceinline__ void write_dx(const Slope<VEC> &slope, const Vec<VEC>
   store_vec<T, VEC>(dx, o.v);
 }
 
-// Gradient, second pass: dx.
+// Gradient, second pass: dx.  As the first 39 us.
 template <typename T, int VEC>
 __global__ void __launch_bounds__(kThreads, sample_blocks(true))
     norm_grad_apply_kernel(const __grid_constant__ NormArgs a) {
@@ -451,7 +454,9 @@ __global__ void __launch_bounds__(kThreads, sample_blocks(true))
 // ------------------------------------------------ samples held by a block
 
 // The block keeps what it read in shared memory; a thread reads back only its
-// own.
+// own.  200 x 300 x 96 bf16 11 us (2.1 TB/s), latency of one turn of the blocks.
+// Clusters of up to 16 blocks that held larger samples together and exchanged sums
+// took 34 us for 64 x 5046 x 64 f16, where two passes take 28.
 template <typename T, int VEC>
 __global__ void __launch_bounds__(kThreads, sample_blocks(false))
     norm_block_kernel(const __grid_constant__ NormArgs a) {
