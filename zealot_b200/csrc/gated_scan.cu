@@ -76,17 +76,27 @@ __device__ __forceinline__ float softplus(float v) {
   return (v > 0.0f ? v : v != v ? v : 0.0f) + 2.0f * z * p;
 }
 
+// What the steps of a stretch need looked at: nothing; marks and the stretch's
+// end; those and rates beyond the series' range.
+enum Way { kPlain, kMarks, kFar };
+template <Way W> using Is = std::integral_constant<Way, W>;
+// Whether scan_kernel has a path of its own for kMarks.  Device us with / without:
+// 1024 x 24 x 512 bf16 32 / 35 (fewer spills), 4096 x 24 x 128 f32 43 / 41.  The fold
+// and the gradient are faster without: 8 x 8191 x 480 bf16 62 / 61 and 128 / 125.
+template <typename T> constexpr bool kMarksApart = sizeof(T) == 2;
+
 // The gates of one step.  With u = rate sigmoid(rec), e = 1 - a = 1 - exp(-u)
 // comes from its series up to u = 0.35 (seven terms, 2e-8 relative): a = 1 - e
 // is then within half a unit of exp(-u) at every step, so the roundings of a
 // long memory do not add up in one direction, and s = 1 - a^2 = e (2 - e)
-// keeps its digits where a is near 1.  Above (only SLOW looks), a comes from
-// ex2.  exp(-rec) may be infinite: sigmoid(rec) and e are then 0.
+// keeps its digits where a is near 1.  Above (only kFar looks), a comes from
+// ex2, so that a small a keeps its digits too, and e = 1 - a from it.  exp(-rec)
+// may be infinite: sigmoid(rec) and e are then 0.
 template <int V>
 struct Decay {
   Vec<V> sr, e, a;  // sigmoid(rec), 1 - a, a
 };
-template <bool SLOW, int V>
+template <Way WAY, int V>
 __device__ __forceinline__ Decay<V> decay(const Vec<V> &rec, const Vec<V> &rate, bool reset) {
   Decay<V> g;
   Vec<V> t = mul(rec, -kLog2e);
@@ -103,15 +113,41 @@ __device__ __forceinline__ Decay<V> decay(const Vec<V> &rec, const Vec<V> &rate,
   p = fma(u, p, -0.5f);
   p = fma(u, p, 1.0f);
   g.e = mul(u, p);
-  if (SLOW) {
+  if (WAY == kMarks && reset) g.e = all<V>(1.0f);
+  g.a = fma(g.e, -1.0f, 1.0f);
+  if (WAY == kFar) {
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      if (u[v] > kSeriesMax) g.e[v] = 1.0f - ex2(u[v] * -kLog2e);
-      if (reset) g.e[v] = 1.0f;  // a = 0, m = 1
+      if (u[v] > kSeriesMax) {
+        g.a[v] = ex2(u[v] * -kLog2e);
+        g.e[v] = 1.0f - g.a[v];
+      }
+      if (reset) g.a[v] = 0.0f, g.e[v] = 1.0f;  // m = 1
     }
   }
-  g.a = fma(g.e, -1.0f, 1.0f);
   return g;
+}
+// a and e in one register a channel, without loss: e up to 1/2, where 1 - e is a
+// to the last bit, else -a (an a of 0 as e = 1).
+template <Way WAY, int V>
+__device__ __forceinline__ Vec<V> hold(const Decay<V> &g) {
+  Vec<V> k = g.e;
+  if (WAY == kFar) {
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      if (g.e[v] > 0.5f && g.a[v] > 0.0f) k[v] = -g.a[v];
+  }
+  return k;
+}
+template <Way WAY, int V>
+__device__ __forceinline__ void held(const Vec<V> &k, Vec<V> &e, Vec<V> &a) {
+  e = k;
+  a = fma(k, -1.0f, 1.0f);
+  if (WAY == kFar) {
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      if (k[v] < 0.0f) a[v] = -k[v], e[v] = 1.0f + k[v];
+  }
 }
 // m sigmoid(inp) = s w with w = 1 / sqrt(s q^2), q = 1 + exp(-inp): one
 // reciprocal square root for the square root and the quotient.  2^-120 on s
@@ -279,8 +315,9 @@ __global__ void __launch_bounds__(256, resident<T>()) scan_fold_kernel(const __g
     const int ahead = (int)max((int64_t)0, min((int64_t)S, steps - t - S));
     const uint32_t z = mark_bits(a, marks, at.one_row);
     marks = marks_of(t + S, ahead);
-    auto run = [&](auto slow, auto more) {
-      constexpr bool SLOW = decltype(slow)::value, MORE = decltype(more)::value;
+    auto run = [&](auto way, auto more) {
+      constexpr Way WAY = decltype(way)::value;
+      constexpr bool SLOW = WAY != kPlain, MORE = decltype(more)::value;
 #pragma unroll
       for (int s = 0; s < S; ++s) {
         if (SLOW && s >= n) break;
@@ -294,7 +331,7 @@ __global__ void __launch_bounds__(256, resident<T>()) scan_fold_kernel(const __g
           if (!BACK) advance(xp, xt, a.one);
         }
         const bool reset = SLOW && (z >> (BACK ? n - 1 - s : s) & 1);
-        const Decay<V> g = decay<SLOW>(r, rate, reset);
+        const Decay<V> g = decay<WAY>(r, rate, reset);
         if (BACK) {
           H = mul(g.a, add(H, i));
           if (reset) H = all<V>(0.0f);
@@ -308,11 +345,11 @@ __global__ void __launch_bounds__(256, resident<T>()) scan_fold_kernel(const __g
       }
     };
     if (big || n < S || (ahead != 0 && ahead != S) || __any_sync(0xffffffffu, z != 0))
-      run(std::true_type{}, std::false_type{});
+      run(Is<kFar>{}, std::false_type{});
     else if (ahead)
-      run(std::false_type{}, std::true_type{});
+      run(Is<kPlain>{}, std::true_type{});
     else
-      run(std::false_type{}, std::false_type{});
+      run(Is<kPlain>{}, std::false_type{});
   }
   let_next_start();
 #pragma unroll
@@ -406,8 +443,9 @@ __global__ void __launch_bounds__(256, resident<T>()) scan_kernel(const __grid_c
         a.carry[(at.b * a.K + t0 / kChunk - 1) * a.D + at.d + v] = h[v];
     }
     // A lane beyond the last channel repeats the last one's steps and stores.
-    auto run = [&](auto slow, auto more) {
-      constexpr bool SLOW = decltype(slow)::value, MORE = decltype(more)::value;
+    auto run = [&](auto way, auto more) {
+      constexpr Way WAY = decltype(way)::value;
+      constexpr bool SLOW = WAY != kPlain, MORE = decltype(more)::value;
 #pragma unroll
       for (int s = 0; s < S; ++s) {
         if (SLOW && s >= n) break;
@@ -421,7 +459,7 @@ __global__ void __launch_bounds__(256, resident<T>()) scan_kernel(const __grid_c
           advance(xp, a.xt, a.one);
         }
         const bool reset = SLOW && (z >> s & 1);
-        const Decay<V> g = decay<SLOW>(r, rate, reset);
+        const Decay<V> g = decay<WAY>(r, rate, reset);
         const Vec<V> b = mul(feed<false>(i, g.e, g.a).ms, x);
         if (reset) h = b;
         else h = fma(g.a, h, b);
@@ -429,12 +467,15 @@ __global__ void __launch_bounds__(256, resident<T>()) scan_kernel(const __grid_c
         advance(hp, a.ht, a.one);
       }
     };
-    if (big || n < S || (ahead != 0 && ahead != S) || __any_sync(0xffffffffu, z != 0))
-      run(std::true_type{}, std::false_type{});
+    const bool marked = n < S || (ahead != 0 && ahead != S) || __any_sync(0xffffffffu, z != 0);
+    if (kMarksApart<T> ? big : big || marked)
+      run(Is<kFar>{}, std::false_type{});
+    else if (kMarksApart<T> && marked)
+      run(Is<kMarksApart<T> ? kMarks : kFar>{}, std::false_type{});
     else if (ahead)
-      run(std::false_type{}, std::true_type{});
+      run(Is<kPlain>{}, std::true_type{});
     else
-      run(std::false_type{}, std::false_type{});
+      run(Is<kPlain>{}, std::false_type{});
   }
   if (a.h_last && slab.index == a.slabs - 1) {
 #pragma unroll
@@ -445,7 +486,7 @@ __global__ void __launch_bounds__(256, resident<T>()) scan_kernel(const __grid_c
 // The gradient, stretch by stretch from a slab's end.  Backwards through a
 // stretch, g_t = dh_t + gamma_{t+1}, gamma_t = a_t g_t, from the decays alone;
 // then forwards, with the states running on from the kept one and every output
-// made as its step comes by.  So every gate is computed once and only 1 - a,
+// made as its step comes by.  So every gate is computed once and only the decay,
 // sigmoid(rec) and g of a stretch are held.  Bound by issue slots (72 a step and
 // channel) at the sixteen warps an SM that its registers allow: 1024 x 24 x 512 bf16
 // 49 us (3.7 TB/s), 8 x 8191 x 480 bf16 125 us (3.6 TB/s).
@@ -517,14 +558,15 @@ __global__ void __launch_bounds__(256, kGradResident)
     t0 -= S;
     n = count(t0);
     marks = load_marks(a, at.b, t0, n, at.one_row);
-    Vec<V> E[S], SR[S], g[S];
+    Vec<V> kept[S], SR[S], g[S];
     auto back = [&](auto tag) {
-      constexpr bool SLOW = decltype(tag)::value;
+      constexpr Way WAY = decltype(tag)::value;
+      constexpr bool SLOW = WAY != kPlain;
 #pragma unroll
       for (int s = S - 1; s >= 0; --s) {
         const bool reset = SLOW && (z >> s & 1);
-        const Decay<V> q = decay<SLOW>(values<T, V>(rr[s]), rate, reset);
-        E[s] = q.e, SR[s] = q.sr;
+        const Decay<V> q = decay<WAY>(values<T, V>(rr[s]), rate, reset);
+        kept[s] = hold<WAY>(q), SR[s] = q.sr;
         g[s] = add(gam, values<T, V>(rg[s]));
         if (!SLOW || s < n_now) {
           gam = mul(q.a, g[s]);
@@ -532,22 +574,24 @@ __global__ void __launch_bounds__(256, kGradResident)
         }
       }
     };
-    if (slow) back(std::true_type{});
-    else back(std::false_type{});
+    if (slow) back(Is<kFar>{});
+    else back(Is<kPlain>{});
     load_back(t0, n);
 
     const char *dx0 = at_step<T>(a.dx, at.b, a.dxb, t_now, a.dxt, at.d);
     const char *dr0 = at_step<T>(a.drec, at.b, a.drb, t_now, a.drt, at.d);
     const char *di0 = at_step<T>(a.dinp, at.b, a.dib, t_now, a.dit, at.d);
     auto finish = [&](auto tag) {
-      constexpr bool SLOW = decltype(tag)::value;
+      constexpr Way WAY = decltype(tag)::value;
+      constexpr bool SLOW = WAY != kPlain;
 #pragma unroll
       for (int s = 0; s < S; ++s) {
         if (SLOW && s >= n_now) break;
         const Vec<V> i = values<T, V>(ri[s]), x = values<T, V>(rx[s]);
         const bool reset = SLOW && (z >> s & 1);
-        const Vec<V> A = fma(E[s], -1.0f, 1.0f);
-        const Feed<V> f = feed<true>(i, E[s], A);
+        Vec<V> e, A;
+        held<WAY>(kept[s], e, A);
+        const Feed<V> f = feed<true>(i, e, A);
         const Vec<V> dx = mul(g[s], f.ms), gx = mul(dx, x);
         // s_i = 1 / q = ms (w q), so dinp = gx (1 - s_i); 1 / s = (w q)^2
         const Vec<V> wq = mul(f.w, f.q);
@@ -571,8 +615,8 @@ __global__ void __launch_bounds__(256, kGradResident)
         advance(di0, a.dit, a.one);
       }
     };
-    if (slow) finish(std::true_type{});
-    else finish(std::false_type{});
+    if (slow) finish(Is<kFar>{});
+    else finish(Is<kPlain>{});
     load_fwd(t0, n);
   }
   let_next_start();
@@ -625,7 +669,7 @@ __global__ void __launch_bounds__(256) scan_step_kernel(const __grid_constant__ 
       const int64_t b = b0 + i * pace;
       if (b >= a.B) break;
       const Vec<V> r = values<T, V>(rr[i]);
-      const Decay<V> g = big || z[i] ? decay<true>(r, rate, z[i] != 0) : decay<false>(r, rate, false);
+      const Decay<V> g = big || z[i] ? decay<kFar>(r, rate, z[i] != 0) : decay<kPlain>(r, rate, false);
       const Vec<V> f =
           mul(feed<false>(values<T, V>(ri[i]), g.e, g.a).ms, values<T, V>(rx[i]));
       const Vec<V> y = z[i] ? f : fma(g.a, h[i], f);
