@@ -28,6 +28,18 @@ struct NormArgs {
   int64_t stretch;
 };
 
+// 1 / (1 + exp(-z))
+template <int V>
+__device__ __forceinline__ Vec<V> sigmoid(const Vec<V> &z) {
+  Vec<V> t = mul(z, -kLog2e);
+#pragma unroll
+  for (int i = 0; i < V; ++i) t[i] = ex2(t[i]);
+  t = add(t, 1.0f);
+#pragma unroll
+  for (int i = 0; i < V; ++i) t[i] = rcp(t[i]);
+  return t;
+}
+
 // Phi(z), the normal distribution's, within 1e-7, and exp(-z^2 / 2): formula
 // 7.1.26 of Abramowitz and Stegun's Handbook (Hastings), erfc(u) = (a1 t + ... +
 // a5 t^5) exp(-u^2) with t = 1 / (1 + p u), at u = |z| / sqrt 2.
@@ -52,49 +64,57 @@ __device__ __forceinline__ Vec<V> normal_cdf(const Vec<V> &z, Vec<V> &e) {
   return add(p, 0.5f);
 }
 
-// act(z).  ELU's and SiLU's exponentials are absolute to 1e-7 of 1, as z itself
-// is of max(1, |z|).
-template <int V>
-__device__ __forceinline__ void act_values(Vec<V> &z, int act) {
+// z becomes act(z), for U vectors at a time so that the branch is taken once for
+// them.  ELU's and SiLU's exponentials are absolute to 1e-7 of 1, as z itself is of
+// max(1, |z|).
+template <int U, int V>
+__device__ __forceinline__ void act_values(Vec<V> (&z)[U], int act) {
   if (act == ZRL_ACT_ELU) {
-    const Vec<V> t = mul(z, kLog2e);
 #pragma unroll
-    for (int i = 0; i < V; ++i) z[i] = z[i] > 0.0f ? z[i] : ex2(t[i]) - 1.0f;
+    for (int u = 0; u < U; ++u) {
+      const Vec<V> t = mul(z[u], kLog2e);
+#pragma unroll
+      for (int i = 0; i < V; ++i) z[u][i] = z[u][i] > 0.0f ? z[u][i] : ex2(t[i]) - 1.0f;
+    }
   } else if (act == ZRL_ACT_SILU) {
-    Vec<V> t = mul(z, -kLog2e);
 #pragma unroll
-    for (int i = 0; i < V; ++i) t[i] = ex2(t[i]);
-    t = add(t, 1.0f);
-#pragma unroll
-    for (int i = 0; i < V; ++i) t[i] = rcp(t[i]);
-    z = mul(z, t);
+    for (int u = 0; u < U; ++u) z[u] = mul(z[u], sigmoid(z[u]));
   } else if (act == ZRL_ACT_GELU) {
-    Vec<V> e;
-    z = mul(z, normal_cdf(z, e));
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      Vec<V> e;
+      z[u] = mul(z[u], normal_cdf(z[u], e));
+    }
   }
 }
 // z becomes act'(z).
-template <int V>
-__device__ __forceinline__ void act_slopes(Vec<V> &z, int act) {
+template <int U, int V>
+__device__ __forceinline__ void act_slopes(Vec<V> (&z)[U], int act) {
   if (act == ZRL_ACT_ELU) {
-    const Vec<V> t = mul(z, kLog2e);
 #pragma unroll
-    for (int i = 0; i < V; ++i) z[i] = z[i] > 0.0f ? 1.0f : ex2(t[i]);
+    for (int u = 0; u < U; ++u) {
+      const Vec<V> t = mul(z[u], kLog2e);
+#pragma unroll
+      for (int i = 0; i < V; ++i) z[u][i] = z[u][i] > 0.0f ? 1.0f : ex2(t[i]);
+    }
   } else if (act == ZRL_ACT_SILU) {
-    Vec<V> t = mul(z, -kLog2e);
 #pragma unroll
-    for (int i = 0; i < V; ++i) t[i] = ex2(t[i]);
-    t = add(t, 1.0f);
-#pragma unroll
-    for (int i = 0; i < V; ++i) t[i] = rcp(t[i]);
-    z = fma(mul(z, t), fma(t, -1.0f, 1.0f), t);
+    for (int u = 0; u < U; ++u) {
+      const Vec<V> t = sigmoid(z[u]);
+      z[u] = fma(mul(z[u], t), fma(t, -1.0f, 1.0f), t);
+    }
   } else if (act == ZRL_ACT_GELU) {
-    Vec<V> e;
-    const Vec<V> p = normal_cdf(z, e);
-    z = fma(mul(z, 0.39894228f), e, p);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      Vec<V> e;
+      const Vec<V> p = normal_cdf(z[u], e);
+      z[u] = fma(mul(z[u], 0.39894228f), e, p);
+    }
   } else {
 #pragma unroll
-    for (int i = 0; i < V; ++i) z[i] = z[i] == z[i] ? 1.0f : z[i];
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < V; ++i) z[u][i] = z[u][i] == z[u][i] ? 1.0f : z[u][i];
   }
 }
 

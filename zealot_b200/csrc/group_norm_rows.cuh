@@ -12,6 +12,14 @@ namespace {
 // single channels: 98304 x 250 f32 forward 62 -> 109 us.
 constexpr int kLaneBlocks = 2;
 
+template <int VEC, int V>
+__device__ __forceinline__ Vec<VEC> slice(const Vec<V> &x, int e) {
+  Vec<VEC> r;
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) r[i] = x[e * VEC + i];
+  return r;
+}
+
 // A thread of the row form: E vectors of VEC channels of one group, the same
 // ones in every row it meets, so its gammas and betas stay in registers.
 template <typename T, int VEC, int E>
@@ -19,7 +27,7 @@ struct RowLanes {
   int r, g;  // row within the block, group
   bool on, lead, has[E];
   int64_t at[E];  // first channel of each vector
-  Vec<VEC> ga[E], be[E];
+  Vec<E * VEC> ga, be;
   __device__ __forceinline__ explicit RowLanes(const NormArgs &a) {
     const int per_row = a.gb * a.p, tid = threadIdx.x;
     r = tid / per_row;
@@ -32,21 +40,36 @@ struct RowLanes {
       const int c = (lane + e * a.p) * VEC;
       has[e] = on && c < a.w;
       at[e] = has[e] ? (int64_t)g * a.w + c : 0;  // a place that can be read
-      ga[e] = has[e] ? params<VEC>(a.gamma, at[e], 1.0f, a.wide) : all<VEC>(0.0f);
-      be[e] = has[e] ? params<VEC>(a.beta, at[e], 0.0f, a.wide) : all<VEC>(0.0f);
+      const Vec<VEC> p = has[e] ? params<VEC>(a.gamma, at[e], 1.0f, a.wide) : all<VEC>(0.0f);
+      const Vec<VEC> q = has[e] ? params<VEC>(a.beta, at[e], 0.0f, a.wide) : all<VEC>(0.0f);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) ga[e * VEC + i] = p[i], be[e * VEC + i] = q[i];
     }
+  }
+  // the lane's channels, vector after vector
+  __device__ __forceinline__ Vec<E * VEC> row(const Raw<T, VEC> (&raw)[E]) const {
+    Vec<E * VEC> r;
+#pragma unroll
+    for (int e = 0; e < E; ++e) unpack<T, VEC>(raw[e], r.v + e * VEC);
+    return r;
+  }
+  __device__ __forceinline__ void write(T *p, const Vec<E * VEC> &x) const {
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (has[e]) store_vec<T, VEC>(p + at[e], x.v + e * VEC);
   }
 };
 
-// U rows rb apart at a time; the next ones' loads are in flight.  Bound by issue
-// slots at the sixteen warps an SM that its registers allow: 24576 x 512 bf16 in
-// groups of 32 ELU 12 us (4.2 TB/s), 98304 x 250 f32 in groups of 25 SiLU 62 us (3.2
-// TB/s: single channels, 55 slots each; rows staged as flat tiles in shared memory
-// took 70).
+// U rows rb apart at a time; the next ones' loads are in flight.  A lane's vectors
+// are taken as one, so that single channels go through the packed instructions
+// too.  Bound by issue slots at the sixteen warps an SM that its registers allow:
+// 24576 x 512 bf16 in groups of 32 ELU 12 us (4.2 TB/s), 98304 x 250 f32 in groups of
+// 25 SiLU 53 us (3.7 TB/s; vector by vector 62, rows staged as flat tiles in shared
+// memory 70).
 template <typename T, int VEC, int E>
 __global__ void __launch_bounds__(kThreads, kLaneBlocks)
     norm_rows_kernel(const __grid_constant__ NormArgs a) {
-  constexpr int U = E * VEC >= 8 ? 2 : 4;
+  constexpr int V = E * VEC, U = V > 8 ? 1 : V == 8 ? 2 : 4;
   const RowLanes<T, VEC, E> k(a);
   const float inv = 1.0f / (float)a.w;
   const int64_t pace = (int64_t)gridDim.x * a.rb * U;
@@ -73,52 +96,47 @@ __global__ void __launch_bounds__(kThreads, kLaneBlocks)
   load(n);
   // the same number of turns for every thread of the block: n - k.r is shared
   for (; n - k.r < a.N; n += pace) {
-    Vec<VEC> x[U][E];
+    Vec<V> x[U];
     float mu[U], rstd[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-#pragma unroll
-      for (int e = 0; e < E; ++e) x[u][e] = values<T, VEC>(raw[u][e]);
-      Vec<VEC> s = x[u][0];  // zero where a lane has no channels
-#pragma unroll
-      for (int e = 1; e < E; ++e) s = add(s, x[u][e]);
-      mu[u] = sum(s);
+      x[u] = k.row(raw[u]);
+      mu[u] = sum(x[u]);  // zero where a lane has no channels
     }
     load(n + pace);
     lanes_sum(mu, a.p);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       mu[u] *= inv;
-      Vec<VEC> q = all<VEC>(0.0f);
+      Vec<V> m;
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        x[u][e] = add(x[u][e], k.has[e] ? -mu[u] : 0.0f);
-        q = fma(x[u][e], x[u][e], q);
-      }
-      rstd[u] = sum(q);
+      for (int i = 0; i < V; ++i) m[i] = k.has[i / VEC] ? -mu[u] : 0.0f;
+      x[u] = add(x[u], m);
+      rstd[u] = sum(mul(x[u], x[u]));
     }
     lanes_sum(rstd, a.p);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      rstd[u] = rsqrtf(fmaf(rstd[u], inv, a.eps));
+      x[u] = fma(x[u], mul(k.ga, rstd[u]), k.be);
+    }
+    act_values(x, a.act);
     T *yr = y0;
 #pragma unroll
     for (int u = 0; u < U; ++u, yr += yu) {
       const int64_t row = n + u * a.rb;
-      const float r = rsqrtf(fmaf(rstd[u], inv, a.eps));
       if (row >= a.N) break;
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        Vec<VEC> z = fma(x[u][e], mul(k.ga[e], r), k.be[e]);
-        act_values<VEC>(z, a.act);
-        if (k.has[e]) store_vec<T, VEC>(yr + k.at[e], z.v);
-      }
+      k.write(yr, x[u]);
       if (k.lead && a.mean) a.mean[row * a.G + k.g] = mu[u];
-      if (k.lead && a.rstd) a.rstd[row * a.G + k.g] = r;
+      if (k.lead && a.rstd) a.rstd[row * a.G + k.g] = rstd[u];
     }
     y0 += pace * a.syn;
   }
 }
 
 // dx, and part[block][2][C]: the block's sums for dgamma and dbeta, kept in
-// registers over all its rows.  98304 x 250 f32 in groups of 25 SiLU 101 us (2.9 TB/s).
+// registers over all its rows.  98304 x 250 f32 in groups of 25 SiLU 101 us (2.9
+// TB/s; 119 with a lane's vectors taken as one: its loads are waited for longer).
 template <typename T, int VEC, int E>
 __global__ void __launch_bounds__(kThreads, kLaneBlocks)
     norm_rows_grad_kernel(const __grid_constant__ NormArgs a) {
@@ -177,14 +195,15 @@ __global__ void __launch_bounds__(kThreads, kLaneBlocks)
       Vec<VEC> t1 = all<VEC>(0.0f), t2 = all<VEC>(0.0f);
 #pragma unroll
       for (int e = 0; e < E; ++e) {
+        const Vec<VEC> ga = slice<VEC>(k.ga, e);
         x[u][e] = mul(add(values<T, VEC>(rx[u][e]), -mu[u]), rs[u]);
-        Vec<VEC> z = fma(x[u][e], k.ga[e], k.be[e]);
-        act_slopes<VEC>(z, a.act);
+        Vec<VEC> z[1] = {fma(x[u][e], ga, slice<VEC>(k.be, e))};
+        act_slopes(z, a.act);
         // zero where a lane has no channels: dy is zero there
-        const Vec<VEC> dz = mul(values<T, VEC>(rd[u][e]), z);
+        const Vec<VEC> dz = mul(values<T, VEC>(rd[u][e]), z[0]);
         db[e] = add(db[e], dz);
         dg[e] = fma(dz, x[u][e], dg[e]);
-        d[u][e] = mul(dz, k.ga[e]);
+        d[u][e] = mul(dz, ga);
         t1 = add(t1, d[u][e]);
         t2 = fma(d[u][e], x[u][e], t2);
       }

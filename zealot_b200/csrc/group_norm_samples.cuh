@@ -162,7 +162,7 @@ struct Nothing {
   __device__ __forceinline__ void operator()() const {}
 };
 // f(raw, count, reload) over the thread's positions, U at a time (count of them in
-// the last turn); f calls reload() when it is done with raw, so that the next
+// the last turn, and zeros after them); f calls reload() when it is done with raw, so that the next
 // ones' loads are in flight while it works.  meanwhile() runs once, by all
 // threads, when the first loads are on their way.
 template <int U, typename T, int VEC, int TENSORS, typename M, typename F>
@@ -182,12 +182,14 @@ __device__ __forceinline__ void each_position(const Patch<VEC> &k, Run<T> (&x)[T
     } else {
 #pragma unroll
       for (int u = 0; u < U; ++u)
-        if (u < n)
 #pragma unroll
-          for (int i = 0; i < TENSORS; ++i) {
+        for (int i = 0; i < TENSORS; ++i) {
+          raw[u][i] = Raw<T, VEC>{};
+          if (u < n) {
             raw[u][i] = *reinterpret_cast<const Raw<T, VEC> *>(x[i].p);
             x[i].next();
           }
+        }
     }
   };
   load(left);
@@ -266,16 +268,22 @@ struct Scale {
     gr = mul(params<VEC>(a.gamma, k.channel(), 1.0f, a.wide), k.of_groups(rstd));
     be = params<VEC>(a.beta, k.channel(), 0.0f, a.wide);
   }
-  template <typename T>
-  __device__ __forceinline__ void write(const Vec<VEC> &x, int act, T *y) const {
-    Vec<VEC> z = fma(add(x, mu), gr, be);
-    act_values<VEC>(z, act);
-    store_vec<T, VEC>(y, z.v);
+  // writes the first count of U positions
+  template <typename T, int U>
+  __device__ __forceinline__ void write(Vec<VEC> (&x)[U], int count, int act, Run<T> &y) const {
+#pragma unroll
+    for (int u = 0; u < U; ++u) x[u] = fma(add(x[u], mu), gr, be);
+    act_values(x, act);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (u < count) store_vec<T, VEC>(y.p, x[u].v);
+      y.next();
+    }
   }
 };
 
 // Second pass: the pieces' means and squares give the group's, then y.  64 x 5046 x
-// 64 f16 ELU 16 us, 16 x 6360 x 256 bf16 GELU 27 us (26 issue slots a value).
+// 64 f16 ELU 16 us, 16 x 6360 x 256 bf16 GELU 27 us (23 issue slots a value).
 template <typename T, int VEC>
 __global__ void __launch_bounds__(kThreads, sample_blocks(false))
     norm_apply_kernel(const __grid_constant__ NormArgs a) {
@@ -322,16 +330,11 @@ __global__ void __launch_bounds__(kThreads, sample_blocks(false))
 #pragma unroll
     for (int u = 0; u < 4; ++u) v[u] = values<T, VEC>(raw[u][0]);
     reload();
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      if (u >= count) break;
-      scale.write(v[u], a.act, y.p);
-      y.next();
-    }
+    scale.write(v, count, a.act, y);
   });
 }
 
-// xh = (x - mu) rstd and dz = dy act'(gamma xh + beta) of a position
+// xh = (x - mu) rstd and dz = dy act'(gamma xh + beta) of U positions
 template <int VEC>
 struct Slope {
   Vec<VEC> mu, rs, ga, be;
@@ -348,12 +351,18 @@ struct Slope {
     ga = params<VEC>(a.gamma, k.channel(), 1.0f, a.wide);
     be = params<VEC>(a.beta, k.channel(), 0.0f, a.wide);
   }
-  __device__ __forceinline__ Vec<VEC> dz(const Vec<VEC> &x, const Vec<VEC> &dy, int act,
-                                         Vec<VEC> &xh) const {
-    xh = mul(add(x, mu), rs);
-    Vec<VEC> z = fma(xh, ga, be);
-    act_slopes<VEC>(z, act);
-    return mul(dy, z);
+  // x becomes xh, dy dz
+  template <int U>
+  __device__ __forceinline__ void dz(Vec<VEC> (&x)[U], Vec<VEC> (&dy)[U], int act) const {
+    Vec<VEC> z[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      x[u] = mul(add(x[u], mu), rs);
+      z[u] = fma(x[u], ga, be);
+    }
+    act_slopes(z, act);
+#pragma unroll
+    for (int u = 0; u < U; ++u) dy[u] = mul(dy[u], z[u]);
   }
 };
 
@@ -408,13 +417,11 @@ __global__ void __launch_bounds__(kThreads, sample_blocks(true))
 #pragma unroll
     for (int u = 0; u < 2; ++u) x[u] = values<T, VEC>(raw[u][0]), d[u] = values<T, VEC>(raw[u][1]);
     reload();
+    slope.dz(x, d, a.act);  // positions after the last have zeros for dy: they add nothing
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      if (u >= count) break;
-      Vec<VEC> xh;
-      const Vec<VEC> dz = slope.dz(x[u], d[u], a.act, xh);
-      db = add(db, dz);
-      dg = fma(dz, xh, dg);
+      db = add(db, d[u]);
+      dg = fma(d[u], x[u], dg);
     }
   });
   let_next_start();
@@ -429,11 +436,12 @@ __global__ void __launch_bounds__(kThreads, sample_blocks(true))
 template <int VEC, typename T>
 __device__ __forceinline__ void write_dx(const Slope<VEC> &slope, const Vec<VEC> &m1,
                                          const Vec<VEC> &m2, const Vec<VEC> &x,
-                                         const Vec<VEC> &dy, int act, T *dx) {
-  Vec<VEC> xh;
-  const Vec<VEC> dz = slope.dz(x, dy, act, xh);
-  const Vec<VEC> o = fma(mul(dz, slope.ga), slope.rs, mul(fma(xh, m2, m1), -1.0f));
-  store_vec<T, VEC>(dx, o.v);
+                                         const Vec<VEC> &dy, int act, Run<T> &dx) {
+  Vec<VEC> xh[1] = {x}, dz[1] = {dy};
+  slope.dz(xh, dz, act);
+  const Vec<VEC> o = fma(mul(dz[0], slope.ga), slope.rs, mul(fma(xh[0], m2, m1), -1.0f));
+  store_vec<T, VEC>(dx.p, o.v);
+  dx.next();
 }
 
 // Gradient, second pass: dx.  As the first 38 us.
@@ -474,8 +482,7 @@ __global__ void __launch_bounds__(kThreads, sample_blocks(true))
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       if (u >= count) break;
-      write_dx(slope, m1, m2, x[u], d[u], a.act, dx.p);
-      dx.next();
+      write_dx(slope, m1, m2, x[u], d[u], a.act, dx);
     }
   });
   let_next_start();
@@ -515,8 +522,11 @@ __global__ void __launch_bounds__(kThreads, sample_blocks(false))
   if (!k.on) return;
   const Scale<VEC> scale(a, k, mu, rstd);
   Run<T> y(a.y, k, a.syn, a.syl);
-  for (int i = 0; i < slot; ++i, y.next())
-    scale.write(values<T, VEC>(kept[i * kThreads]), a.act, y.p);
+  for (int i = 0; i < slot; i += 2) {
+    Vec<VEC> v[2] = {values<T, VEC>(kept[i * kThreads]),
+                     values<T, VEC>(kept[(i + 1 < slot ? i + 1 : i) * kThreads])};
+    scale.write(v, slot - i, a.act, y);
+  }
 }
 
 template <typename T, int VEC>
@@ -541,13 +551,11 @@ __global__ void __launch_bounds__(kThreads, sample_blocks(true))
       }
     }
     reload();
+    slope.dz(x, d, a.act);  // positions after the last have zeros for dy: they add nothing
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      if (u >= count) break;
-      Vec<VEC> xh;
-      const Vec<VEC> dz = slope.dz(x[u], d[u], a.act, xh);
-      db = add(db, dz);
-      dg = fma(dz, xh, dg);
+      db = add(db, d[u]);
+      dg = fma(d[u], x[u], dg);
     }
   });
   let_next_start();
@@ -558,9 +566,9 @@ __global__ void __launch_bounds__(kThreads, sample_blocks(true))
   const Vec<VEC> m1 = mul(mul(k.of_groups(s1), inv), slope.rs);
   const Vec<VEC> m2 = mul(mul(k.of_groups(s2), inv), slope.rs);
   Run<T> dx(a.dx, k, a.sdn, a.sdl);
-  for (int i = 0; i < slot; ++i, dx.next())
+  for (int i = 0; i < slot; ++i)
     write_dx(slope, m1, m2, values<T, VEC>(kept[2 * i * kThreads]),
-             values<T, VEC>(kept[(2 * i + 1) * kThreads]), a.act, dx.p);
+             values<T, VEC>(kept[(2 * i + 1) * kThreads]), a.act, dx);
 }
 
 }  // namespace

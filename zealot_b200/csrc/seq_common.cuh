@@ -131,46 +131,43 @@ __device__ __forceinline__ Vec<V> all(float c) {
 template <int V>
 __device__ __forceinline__ Vec<V> fma(const Vec<V> &a, const Vec<V> &b, const Vec<V> &c) {
   Vec<V> r;
-  if constexpr (V % 2 == 0) {
 #pragma unroll
-    for (int i = 0; i < V; i += 2) {
-      const float2 f = __ffma2_rn(make_float2(a[i], a[i + 1]), make_float2(b[i], b[i + 1]),
-                                  make_float2(c[i], c[i + 1]));
-      r[i] = f.x, r[i + 1] = f.y;
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < V; ++i) r[i] = fmaf(a[i], b[i], c[i]);
+  for (int i = 0; i + 1 < V; i += 2) {
+    const float2 f = __ffma2_rn(make_float2(a[i], a[i + 1]), make_float2(b[i], b[i + 1]),
+                                make_float2(c[i], c[i + 1]));
+    r[i] = f.x, r[i + 1] = f.y;
+  }
+  if constexpr (V % 2) {
+    constexpr int i = V - 1;
+    r[i] = fmaf(a[i], b[i], c[i]);
   }
   return r;
 }
 template <int V>
 __device__ __forceinline__ Vec<V> mul(const Vec<V> &a, const Vec<V> &b) {
   Vec<V> r;
-  if constexpr (V % 2 == 0) {
 #pragma unroll
-    for (int i = 0; i < V; i += 2) {
-      const float2 f = __fmul2_rn(make_float2(a[i], a[i + 1]), make_float2(b[i], b[i + 1]));
-      r[i] = f.x, r[i + 1] = f.y;
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < V; ++i) r[i] = a[i] * b[i];
+  for (int i = 0; i + 1 < V; i += 2) {
+    const float2 f = __fmul2_rn(make_float2(a[i], a[i + 1]), make_float2(b[i], b[i + 1]));
+    r[i] = f.x, r[i + 1] = f.y;
+  }
+  if constexpr (V % 2) {
+    constexpr int i = V - 1;
+    r[i] = a[i] * b[i];
   }
   return r;
 }
 template <int V>
 __device__ __forceinline__ Vec<V> add(const Vec<V> &a, const Vec<V> &b) {
   Vec<V> r;
-  if constexpr (V % 2 == 0) {
 #pragma unroll
-    for (int i = 0; i < V; i += 2) {
-      const float2 f = __fadd2_rn(make_float2(a[i], a[i + 1]), make_float2(b[i], b[i + 1]));
-      r[i] = f.x, r[i + 1] = f.y;
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < V; ++i) r[i] = a[i] + b[i];
+  for (int i = 0; i + 1 < V; i += 2) {
+    const float2 f = __fadd2_rn(make_float2(a[i], a[i + 1]), make_float2(b[i], b[i + 1]));
+    r[i] = f.x, r[i + 1] = f.y;
+  }
+  if constexpr (V % 2) {
+    constexpr int i = V - 1;
+    r[i] = a[i] + b[i];
   }
   return r;
 }
@@ -198,6 +195,11 @@ template <int V>
 __device__ __forceinline__ float sum(const Vec<V> &a) {
   if constexpr (V == 1) {
     return a[0];
+  } else if constexpr (V % 2) {
+    Vec<V - 1> h;
+#pragma unroll
+    for (int i = 0; i < V - 1; ++i) h[i] = a[i];
+    return sum(h) + a[V - 1];
   } else {
     Vec<V / 2> h, l;
 #pragma unroll
