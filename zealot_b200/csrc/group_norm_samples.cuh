@@ -15,8 +15,9 @@ namespace {
 
 // Channels a thread has at most, and blocks an SM holds, which bounds their
 // registers: eight channels at two blocks are as fast within a tenth (64 x 5046 x
-// 64 f16 forward 28 and 28 us, 16 x 6360 x 256 bf16 GELU with gradient 124 and 126),
-// two channels at six blocks slower (36 and 156).
+// 64 f16 forward 28 and 28 us, 16 x 6360 x 256 bf16 GELU with gradient 124 and 126,
+// before the blocks' sums were taken by teams), two channels at six blocks slower
+// (36 and 156).
 constexpr int kMaxChannels = 4;
 constexpr int sample_blocks(bool grad) { return grad ? 3 : 4; }
 
@@ -402,7 +403,7 @@ __device__ __forceinline__ void grad_sums(const NormArgs &a, const Patch<VEC> &k
 }
 
 // Gradient, first pass: grad_sums, the groups' into means[n][group][piece].  16 x
-// 6360 x 256 bf16 GELU 32 us (3.2 TB/s; 31 without the block's sums, and no more
+// 6360 x 256 bf16 GELU 33 us (3.1 TB/s; 31 without the block's sums, and no more
 // without the GELU); four positions a turn take as long.
 template <typename T, int VEC>
 __global__ void __launch_bounds__(kThreads, sample_blocks(true))
