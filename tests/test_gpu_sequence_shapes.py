@@ -97,3 +97,22 @@ def test_dropout_widths(D, t):
     mask = keep_mask(np.arange(37), D, 0.3, 123, 9)
     want, slack = expected(x, mask, 0.3, x)
     assert_within(S.dropout(x, 0.3, 123, stream=9, residual=x), want, slack)
+
+
+# A constant sample whose (0 - mean) rstd is infinite, which nothing but the
+# sample's own positions may show (the statistics are given: fp32 sums of so large
+# values overflow).  xh is 0 everywhere, so dgamma is 0 and dbeta the sum of
+# dy act'(0).
+@pytest.mark.parametrize("L", [1, 3, 301, 5001])
+@pytest.mark.parametrize("act", ["none", "silu", "gelu"])
+def test_norm_gradient_of_a_huge_constant(L, act):
+    C = 64
+    x = torch.full((2, L, C), 2.0 ** 120, device="cuda")
+    dy = torch.ones_like(x)
+    ones, zeros = torch.ones(C, device="cuda"), torch.zeros(C, device="cuda")
+    mean, rstd = torch.full((2, 8), 2.0 ** 120, device="cuda"), torch.full((2, 8), 316.0, device="cuda")
+    dx, dgamma, dbeta = S.group_norm_grad(x, dy, 8, ones, zeros, mean, rstd, act=act)
+    assert torch.equal(dgamma, zeros)
+    slope = 1.0 if act == "none" else 0.5
+    assert torch.allclose(dbeta, torch.full_like(dbeta, 2 * L * slope), rtol=1e-6 * (1 + L ** 0.5))
+    assert torch.isfinite(dx).all()

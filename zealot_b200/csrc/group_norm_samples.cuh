@@ -418,9 +418,10 @@ __global__ void __launch_bounds__(kThreads, sample_blocks(true))
 #pragma unroll
     for (int u = 0; u < 2; ++u) x[u] = values<T, VEC>(raw[u][0]), d[u] = values<T, VEC>(raw[u][1]);
     reload();
-    slope.dz(x, d, a.act);  // positions after the last have zeros for dy: they add nothing
+    slope.dz(x, d, a.act);
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
+      if (u >= count) break;  // a filled position may be NaN: (0 - mean) rstd may be infinite
       db = add(db, d[u]);
       dg = fma(d[u], x[u], dg);
     }
@@ -552,9 +553,10 @@ __global__ void __launch_bounds__(kThreads, sample_blocks(true))
       }
     }
     reload();
-    slope.dz(x, d, a.act);  // positions after the last have zeros for dy: they add nothing
+    slope.dz(x, d, a.act);
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
+      if (u >= count) break;  // a filled position may be NaN: (0 - mean) rstd may be infinite
       db = add(db, d[u]);
       dg = fma(d[u], x[u], dg);
     }
