@@ -163,7 +163,8 @@ struct Nothing {
   __device__ __forceinline__ void operator()() const {}
 };
 // f(raw, count, reload) over the thread's positions, U at a time (count of them in
-// the last turn, and zeros after them); f calls reload() when it is done with raw, so that the next
+// the last turn; after them the first one's x again, whose (x - mean) rstd is as
+// finite as the data, and zeros for dy); f calls reload() when it is done with raw, so that the next
 // ones' loads are in flight while it works.  meanwhile() runs once, by all
 // threads, when the first loads are on their way.
 template <int U, typename T, int VEC, int TENSORS, typename M, typename F>
@@ -185,7 +186,7 @@ __device__ __forceinline__ void each_position(const Patch<VEC> &k, Run<T> (&x)[T
       for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int i = 0; i < TENSORS; ++i) {
-          raw[u][i] = Raw<T, VEC>{};
+          raw[u][i] = i == 0 && u > 0 ? raw[0][0] : Raw<T, VEC>{};
           if (u < n) {
             raw[u][i] = *reinterpret_cast<const Raw<T, VEC> *>(x[i].p);
             x[i].next();
@@ -418,10 +419,9 @@ __global__ void __launch_bounds__(kThreads, sample_blocks(true))
 #pragma unroll
     for (int u = 0; u < 2; ++u) x[u] = values<T, VEC>(raw[u][0]), d[u] = values<T, VEC>(raw[u][1]);
     reload();
-    slope.dz(x, d, a.act);
+    slope.dz(x, d, a.act);  // positions after the last have zeros for dy: they add nothing
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      if (u >= count) break;  // a filled position may be NaN: (0 - mean) rstd may be infinite
       db = add(db, d[u]);
       dg = fma(d[u], x[u], dg);
     }
@@ -553,10 +553,9 @@ __global__ void __launch_bounds__(kThreads, sample_blocks(true))
       }
     }
     reload();
-    slope.dz(x, d, a.act);
+    slope.dz(x, d, a.act);  // positions after the last have zeros for dy: they add nothing
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      if (u >= count) break;  // a filled position may be NaN: (0 - mean) rstd may be infinite
       db = add(db, d[u]);
       dg = fma(d[u], x[u], dg);
     }
