@@ -196,7 +196,8 @@ __global__ void __launch_bounds__(kThreads, kLaneBlocks)
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         const Vec<VEC> ga = slice<VEC>(k.ga, e);
-        x[u][e] = mul(add(values<T, VEC>(rx[u][e]), -mu[u]), rs[u]);
+        // no mean where a lane has no channels: (0 - mean) rstd may be infinite
+        x[u][e] = mul(add(values<T, VEC>(rx[u][e]), k.has[e] ? -mu[u] : 0.0f), rs[u]);
         Vec<VEC> z[1] = {fma(x[u][e], ga, slice<VEC>(k.be, e))};
         act_slopes(z, a.act);
         // zero where a lane has no channels: dy is zero there
