@@ -1,5 +1,7 @@
 """Group norm where digits or finiteness are easily lost: lanes without channels of
-their own, activations near zero.  Bounds in e = 2^-24."""
+their own, activations near zero and in their tails.  Bounds in e = 2^-24."""
+import math
+
 import pytest
 import torch
 
@@ -80,3 +82,18 @@ def test_elu_under_a_small_gamma(shape, groups, scale):
     want = torch.where(z > 0, z, torch.expm1(z))
     slack = d_xh.reshape(shape) * gamma.double() + 18 * EPS * want.abs()
     assert_within(y, want, slack, f"gamma {scale}")
+
+
+# The tail of Phi keeps its digits: e^(-z^2/2) has its argument's rounding, z^2 e,
+# and the factor beside it is within 8 e with its division and products, 16 more.
+@pytest.mark.gpu
+@pytest.mark.parametrize("N,L", FORMS)
+def test_gelu_keeps_the_digits_of_the_tail(N, L):
+    z = torch.cat([torch.linspace(-12, 12, 1007), torch.tensor([0.0] + [1e-3, -1e-3, 1e-20, -1e-20] * 4)])
+    y, slope = direct(z, "gelu", N, L)
+    z = z.double()
+    rel = (32 + z * z) * EPS
+    phi = torch.special.erfc(-z / math.sqrt(2)) / 2
+    e = torch.exp(-z * z / 2) / math.sqrt(2 * math.pi)
+    assert_within(y, (z * phi).expand(y.shape), rel * (z * phi).abs(), "y")
+    assert_within(slope, phi + z * e, rel * (phi + z.abs() * e), "slope")
