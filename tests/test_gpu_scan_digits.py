@@ -1,0 +1,42 @@
+"""Where the gated scan's digits go: gates nearly shut."""
+import pytest
+import torch
+
+import test_gpu_gated_scan as G
+from seq_helpers import EPS, TYPES, assert_within
+from zealot_b200 import sequence as S
+
+pytestmark = pytest.mark.gpu
+INF = float("inf")
+
+
+# The bounds of the operator's own tests are relative to each step's input
+# sqrt(1 - a^2) sigmoid(inp) x, so a gate that is nearly shut has to be as exact as
+# an open one; from a state of zero nothing larger hides it.
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+@pytest.mark.parametrize("T", [1, 5, 24, 200])
+@pytest.mark.parametrize("gate", ["inp", "rec"])
+def test_gates_nearly_shut(gate, T, t):
+    D = 176
+    kw, dh, dh_last = G.make(3, T, D, t, seed=9, resets=0, h0=False)
+    at = torch.cat([torch.linspace(-72, 72, D - 16), torch.tensor([-INF, INF, -45.0, -41.6, 0.0, -60.0, -70.0, 40.0] * 2)])
+    kw[gate] = at.to(TYPES[t]).cuda().expand(3, T, D).contiguous()
+    G.check(kw, dh, dh_last, what=gate)
+    # every state of its own: a step's input alone
+    kw["resets"] = torch.ones(3, T, dtype=torch.uint8, device="cuda")
+    G.check(kw, dh, dh_last, what=gate + " apart")
+
+
+@pytest.mark.parametrize("T", [1, 24, 200])
+def test_a_shut_gate_lets_nothing_in(T):
+    kw, dh, dh_last = G.make(2, T, 64, "f32", resets=0, h0=False)
+    for gate in ("inp", "rec"):
+        k = dict(kw)
+        k[gate] = torch.full_like(kw[gate], -INF)
+        h, last, carry = S.gated_scan(**k, save=True)
+        assert not h.any() and not last.any()
+        dx, drec, dinp, dlam, _ = S.gated_scan_grad(k["x"], k["rec"], k["inp"], k["lam"], dh, carry,
+                                                    dh_last=dh_last)
+        assert not dx.any() and not dinp.any()
+        if gate == "rec":
+            assert not drec.any() and not dlam.any()

@@ -26,7 +26,7 @@ constexpr int kMinSlab = 16;    // steps of a slab at least
 // gradient recomputes the states inside a stretch from there.
 constexpr int kChunk = kSteps;
 constexpr float kSeriesMax = 0.35f;
-constexpr float kTinySquare = 7.5231638e-37f;  // 2^-120
+constexpr float kSmallest = 1.17549435e-38f;  // 2^-126
 
 // Blocks of 256 threads an SM holds, which bounds their registers.  Measured
 // (device us, 2 / 3 / 4 blocks): forward 1024 x 24 x 512 bf16 35 / 34 / 32, 4096 x
@@ -51,13 +51,6 @@ struct ScanArgs {
   float c;
   int32_t one;  // 1
 };
-
-// NaN stays NaN, unlike fminf
-__device__ __forceinline__ float min_nan(float a, float b) {
-  float r;
-  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
 
 // softplus(v) = max(v, 0) + log(1 + y), y = exp(-|v|), with
 // log(1 + y) = 2 artanh(z), z = y / (2 + y) <= 1/3: its series to z^15 is within
@@ -149,27 +142,31 @@ __device__ __forceinline__ void held(const Vec<V> &k, Vec<V> &e, Vec<V> &a) {
       if (k[v] < 0.0f) a[v] = -k[v], e[v] = 1.0f + k[v];
   }
 }
-// m sigmoid(inp) = s w with w = 1 / sqrt(s q^2), q = 1 + exp(-inp): one
-// reciprocal square root for the square root and the quotient.  2^-120 on s
-// keeps w finite where a is 1; q may be infinite (w and m sigmoid(inp) are then
-// 0) unless HELD, which holds it to 2^60 for the products of w and q.
+// s = 1 - a^2 and sigmoid(inp), each to a few units in its last place however nearly
+// shut its gate: a reciprocal and a root of their own.  (One reciprocal square root of
+// s (1 + exp(-inp))^2 for both overflows from inp = -45 down, and needs s held above 0.)
+// exp(-inp) may be infinite: sigmoid(inp) is then 0.
 template <int V>
-struct Feed {
-  Vec<V> ms, w, q;
-};
-template <bool HELD, int V>
-__device__ __forceinline__ Feed<V> feed(const Vec<V> &inp, const Vec<V> &e, const Vec<V> &a) {
-  Feed<V> f;
+__device__ __forceinline__ Vec<V> square(const Vec<V> &e, const Vec<V> &a) {
+  return mul(e, add(a, 1.0f));
+}
+template <int V>
+__device__ __forceinline__ Vec<V> gate(const Vec<V> &inp) {
   Vec<V> t = mul(inp, -kLog2e);
 #pragma unroll
-  for (int v = 0; v < V; ++v) t[v] = ex2(HELD ? min_nan(t[v], 60.0f) : t[v]);
-  f.q = add(t, 1.0f);
-  const Vec<V> s = fma(e, add(a, 1.0f), kTinySquare);
-  t = mul(mul(s, f.q), f.q);
+  for (int v = 0; v < V; ++v) t[v] = ex2(t[v]);
+  t = add(t, 1.0f);
 #pragma unroll
-  for (int v = 0; v < V; ++v) f.w[v] = rsq(t[v]);
-  f.ms = mul(s, f.w);
-  return f;
+  for (int v = 0; v < V; ++v) t[v] = rcp(t[v]);
+  return t;
+}
+// m sigmoid(inp)
+template <int V>
+__device__ __forceinline__ Vec<V> feed(const Vec<V> &inp, const Vec<V> &e, const Vec<V> &a) {
+  Vec<V> m = square(e, a);
+#pragma unroll
+  for (int v = 0; v < V; ++v) m[v] = root(m[v]);
+  return mul(m, gate(inp));
 }
 
 // A stretch of steps maps the state before it to h -> P h + H.  P is -0 where
@@ -336,7 +333,7 @@ __global__ void __launch_bounds__(256, resident<T>()) scan_fold_kernel(const __g
           H = mul(g.a, add(H, i));
           if (reset) H = all<V>(0.0f);
         } else {
-          const Vec<V> b = mul(feed<false>(i, g.e, g.a).ms, x);
+          const Vec<V> b = mul(feed(i, g.e, g.a), x);
           if (reset) H = b;
           else H = fma(g.a, H, b);
         }
@@ -460,7 +457,7 @@ __global__ void __launch_bounds__(256, resident<T>()) scan_kernel(const __grid_c
         }
         const bool reset = SLOW && (z >> s & 1);
         const Decay<V> g = decay<WAY>(r, rate, reset);
-        const Vec<V> b = mul(feed<false>(i, g.e, g.a).ms, x);
+        const Vec<V> b = mul(feed(i, g.e, g.a), x);
         if (reset) h = b;
         else h = fma(g.a, h, b);
         store_step<T, V>(hp, h);
@@ -591,20 +588,22 @@ __global__ void __launch_bounds__(256, kGradResident)
         const bool reset = SLOW && (z >> s & 1);
         Vec<V> e, A;
         held<WAY>(kept[s], e, A);
-        const Feed<V> f = feed<true>(i, e, A);
-        const Vec<V> dx = mul(g[s], f.ms), gx = mul(dx, x);
-        // s_i = 1 / q = ms (w q), so dinp = gx (1 - s_i); 1 / s = (w q)^2
-        const Vec<V> wq = mul(f.w, f.q);
-        const Vec<V> gms = mul(gx, mul(f.ms, wq));
-        const Vec<V> dinp = fma(gms, -1.0f, gx);
-        // q = g (h a - s_i x a^2 / m) = a (g h - g m s_i x a / s)
-        Vec<V> q = mul(mul(gx, A), mul(wq, wq));
+        // 1 / m, kept finite where m is 0, so that nothing comes of it there
+        const Vec<V> sq_m = square(e, A), si = gate(i);
+        Vec<V> inv_m;
+#pragma unroll
+        for (int v = 0; v < V; ++v) inv_m[v] = rsq(fmaxf(sq_m[v], kSmallest));
+        const Vec<V> ms = mul(mul(sq_m, inv_m), si);
+        const Vec<V> dx = mul(g[s], ms), gx = mul(dx, x);
+        const Vec<V> dinp = fma(mul(gx, si), -1.0f, gx);
+        // q = g (h a - s_i x a^2 / m) = a (g h - g m s_i x a / m^2)
+        Vec<V> q = mul(mul(gx, A), mul(inv_m, inv_m));
         q = mul(A, fma(q, -1.0f, mul(g[s], h)));
         if (reset) q = all<V>(0.0f);
         const Vec<V> sq = mul(SR[s], q);
         const Vec<V> drec = mul(mul(rate, add(SR[s], -1.0f)), sq);
         dl = add(dl, sq);
-        const Vec<V> b = mul(f.ms, x);
+        const Vec<V> b = mul(ms, x);
         if (reset) h = b;
         else h = fma(A, h, b);
         store_step<T, V>(dx0, dx);
@@ -671,7 +670,7 @@ __global__ void __launch_bounds__(256) scan_step_kernel(const __grid_constant__ 
       const Vec<V> r = values<T, V>(rr[i]);
       const Decay<V> g = big || z[i] ? decay<kFar>(r, rate, z[i] != 0) : decay<kPlain>(r, rate, false);
       const Vec<V> f =
-          mul(feed<false>(values<T, V>(ri[i]), g.e, g.a).ms, values<T, V>(rx[i]));
+          mul(feed(values<T, V>(ri[i]), g.e, g.a), values<T, V>(rx[i]));
       const Vec<V> y = z[i] ? f : fma(g.a, h[i], f);
       store_step<T, V>(at_step<T>(a.h, b, a.hb, 0, 0, d), y);
       if (a.h_last) {

@@ -96,8 +96,8 @@ __device__ __forceinline__ Raw<T, V> pack(const float *in) {
 
 constexpr float kLog2e = 1.44269504f;
 
-// The special functions' approximate forms: 2^v, 1 / v and 1 / sqrt(v) within a
-// few units in the last place (PTX's stated bounds), subnormals as zero.
+// The special functions' approximate forms: 2^v, 1 / v, 1 / sqrt(v) and sqrt(v)
+// within a few units in the last place (PTX's stated bounds), subnormals as zero.
 __device__ __forceinline__ float ex2(float v) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
@@ -111,6 +111,11 @@ __device__ __forceinline__ float rcp(float v) {
 __device__ __forceinline__ float rsq(float v) {
   float r;
   asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float root(float v) {
+  float r;
+  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
   return r;
 }
 // V channels' values.  Pairs go through the packed fp32 instructions, which
