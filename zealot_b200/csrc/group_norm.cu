@@ -220,10 +220,12 @@ zrl_status check_norm(const char *what, int64_t N, int64_t L, int64_t C, int32_t
 // The launch error, if any, is left for cudaGetLastError.
 void launch_norm(void (*kernel)(NormArgs), dim3 grid, const NormPlan &p, cudaStream_t st,
                  const NormArgs &a) {
-  // up to 48 KB, with up to 24 KB of static memory beside it, need no leave
+  // up to 48 KB, with up to 24 KB of static memory beside it, need no leave.  The limit
+  // is the whole context's, so it is always the most that any call takes: a call from
+  // another thread never lowers it between here and the launch.
   if (p.bytes > (24 << 10) &&
-      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)p.bytes) !=
-          cudaSuccess)
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           (int)kBlockBytes) != cudaSuccess)
     return;
   kernel<<<grid, kThreads, (size_t)p.bytes, st>>>(a);
 }
