@@ -1,4 +1,4 @@
-"""Where the gated scan's digits go: gates nearly shut."""
+"""Where the gated scan's digits go: gates nearly shut, and sums over a long row."""
 import pytest
 import torch
 
@@ -40,3 +40,28 @@ def test_a_shut_gate_lets_nothing_in(T):
         assert not dx.any() and not dinp.any()
         if gate == "rec":
             assert not drec.any() and not dlam.any()
+
+
+# dlam of a long row that one thread sums: as many rows as keep rows in one piece,
+# all alike, so that every term has the same value and a single running sum errs to
+# one side by up to T / 2 roundings.  Sums of 256 terms, then of those, and of the
+# rows: 256 + T / 256 + 60 roundings, on top of the terms' own bound.
+def test_dlam_of_a_long_row_in_one_piece():
+    B, T, D = 592, 32768, 64
+    g = torch.Generator().manual_seed(4)
+    row = {k: torch.randn(D, generator=g) for k in ("x", "rec", "inp", "dh")}
+    row["x"], row["dh"] = 1 + row["x"].abs(), 1 + row["dh"].abs()
+    lam = torch.log(torch.expm1(0.17 + 0.1 * torch.rand(D, generator=g)))
+    want, slack = G.reference(*(row[k].expand(1, T, D) for k in ("x", "rec", "inp")), lam,
+                              dh=row["dh"].expand(1, T, D))["dlam"]
+    x, rec, inp, dh = (row[k].cuda().expand(B, T, D) for k in ("x", "rec", "inp", "dh"))
+    carry = S.gated_scan(x, rec, inp, lam.cuda(), save=True)[2]
+    dlam = S.gated_scan_grad(x, rec, inp, lam.cuda(), dh, carry)[3]
+    assert_within(dlam, B * want, B * (slack + (256 + T / 256 + 60) * EPS * want.abs()), "dlam")
+
+
+# A row in one piece through hundreds of stretches, the last one short.
+@pytest.mark.parametrize("t,B,T,D", [("f32", 592, 1001, 64), ("bf16", 1300, 1003, 66)])
+def test_long_rows_in_one_piece(t, B, T, D):
+    kw, dh, dh_last = G.make(B, T, D, t, seed=8, resets=0.005)
+    G.check(kw, dh, dh_last, what=f"{B}x{T}x{D} {t}")

@@ -25,6 +25,7 @@ constexpr int kMinSlab = 16;    // steps of a slab at least
 // The forward call keeps the state before every stretch after the first; the
 // gradient recomputes the states inside a stretch from there.
 constexpr int kChunk = kSteps;
+constexpr int kRun = 256;       // steps whose terms of dlam are summed one after the other
 constexpr float kSeriesMax = 0.35f;
 constexpr float kSmallest = 1.17549435e-38f;  // 2^-126
 
@@ -540,7 +541,7 @@ __global__ void __launch_bounds__(256, kGradResident)
   load_back(t0, n);
   load_fwd(t0, n);
   uint32_t marks = load_marks(a, at.b, t0, n, at.one_row);
-  Vec<V> rate, gam, dl = all<V>(0.0f);
+  Vec<V> rate, gam, dl = all<V>(0.0f), runs = dl;  // dlam's sum of this run, of the runs
 #pragma unroll
   for (int v = 0; v < V; ++v)
     gam[v] = a.dh_last ? a.dh_last[at.b * a.D + at.d + v] : 0.0f;
@@ -617,12 +618,14 @@ __global__ void __launch_bounds__(256, kGradResident)
     if (slow) finish(Is<kFar>{});
     else finish(Is<kPlain>{});
     load_fwd(t0, n);
+    if (t_now % kRun == 0) runs = add(runs, dl), dl = all<V>(0.0f);
   }
+  runs = add(runs, dl);
   let_next_start();
   if (at.live && slab.index < a.slabs) {
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      a.part[((int64_t)slab.index * a.B + at.b) * a.D + at.d + v] = dl[v];
+      a.part[((int64_t)slab.index * a.B + at.b) * a.D + at.d + v] = runs[v];
       if (a.dh0 && slab.index == 0) a.dh0[at.b * a.D + at.d + v] = gam[v];
     }
   }
