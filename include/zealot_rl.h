@@ -135,7 +135,8 @@ zrl_status zrl_create(const zrl_model_config *cfg, int device,
 zrl_status zrl_destroy(zrl_ctx *ctx);
 /* The message of the last failure on ctx (where the reference panics, this
  * library returns a status and keeps the message here).  With ctx NULL: the
- * message of the calling thread's last failed sequence-operator call. */
+ * message of the calling thread's last failed sequence-operator call, or "null
+ * context" if there is none or a call that was given no context came after. */
 const char *zrl_last_error(const zrl_ctx *ctx);
 /* ZRL_ABI_VERSION of the loaded library.  No counterpart in the reference. */
 int32_t zrl_abi_version(void);

@@ -24,5 +24,6 @@ zrl_status seq_launched(const char *what) {
 }
 
 const char *seq_last_error() { return g_msg; }
+void seq_clear_error() { g_msg[0] = 0; }
 
 }  // namespace zrl

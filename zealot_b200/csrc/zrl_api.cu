@@ -1433,6 +1433,13 @@ static zrl_status prof_end(zrl_ctx *ctx, cudaEvent_t u0) {
 
 // =================================================================== ABI
 
+// No context was given: zrl_last_error(NULL) then says so, and not what an earlier
+// sequence operator said.
+static bool absent(const zrl_ctx *ctx) {
+  if (!ctx) seq_clear_error();
+  return !ctx;
+}
+
 extern "C" {
 
 int32_t zrl_abi_version(void) { return ZRL_ABI_VERSION; }
@@ -1453,6 +1460,7 @@ const char *zrl_last_error(const zrl_ctx *ctx) {
 
 zrl_status zrl_create(const zrl_model_config *cfg, int device,
                       const zrl_comm *comm, zrl_ctx **out) {
+  seq_clear_error();  // there is no context to keep a message
   if (!cfg || !out) return ZRL_INVALID_ARG;
   *out = nullptr;
   if (cfg->n_actor_dims < 2 || cfg->n_critic_dims < 2 ||
@@ -1583,7 +1591,7 @@ zrl_status zrl_destroy(zrl_ctx *ctx) {
 }
 
 zrl_status zrl_synchronize(zrl_ctx *ctx) {
-  if (!ctx) return ZRL_INVALID_ARG;
+  if (absent(ctx)) return ZRL_INVALID_ARG;
   CK(cudaStreamSynchronize(ctx->stream));
   return ZRL_OK;
 }
@@ -1603,7 +1611,7 @@ static zrl_status reset_adam(zrl_ctx *ctx) {
 }
 
 zrl_status zrl_set_params(zrl_ctx *ctx, const float *flat, int64_t count) {
-  if (!ctx || !flat) return ZRL_INVALID_ARG;
+  if (absent(ctx) || !flat) return ZRL_INVALID_ARG;
   if (count != ctx->flat_params) return bad(ctx, "parameter count mismatch");
   CK(cudaSetDevice(ctx->device));
   std::vector<float> pad(ctx->dev_params);
@@ -1621,7 +1629,7 @@ zrl_status zrl_set_params(zrl_ctx *ctx, const float *flat, int64_t count) {
 }
 
 zrl_status zrl_get_params(zrl_ctx *ctx, float *flat, int64_t count) {
-  if (!ctx || !flat) return ZRL_INVALID_ARG;
+  if (absent(ctx) || !flat) return ZRL_INVALID_ARG;
   if (count != ctx->flat_params) return bad(ctx, "parameter count mismatch");
   CK(cudaSetDevice(ctx->device));
   std::vector<float> pad(ctx->dev_params);
@@ -1634,7 +1642,7 @@ zrl_status zrl_get_params(zrl_ctx *ctx, float *flat, int64_t count) {
 
 zrl_status zrl_init_reference(zrl_ctx *ctx, float init_noise_std, float init_lr,
                               uint64_t *lcg_state) {
-  if (!ctx || !lcg_state || !(init_noise_std > 0.0f)) return ZRL_INVALID_ARG;
+  if (absent(ctx) || !lcg_state || !(init_noise_std > 0.0f)) return ZRL_INVALID_ARG;
   std::vector<float> flat(ctx->flat_params);
   const NetLayout &La = ctx->net[0], &Lc = ctx->net[1];
   mlp_init_reference(ctx->mcfg.actor_dims, ctx->mcfg.n_actor_dims, 0.01f, lcg_state,
@@ -1649,7 +1657,7 @@ zrl_status zrl_init_reference(zrl_ctx *ctx, float init_noise_std, float init_lr,
 
 zrl_status zrl_set_adam_state(zrl_ctx *ctx, const int32_t *t3, const float *m,
                               const float *v, int64_t count) {
-  if (!ctx || !t3) return ZRL_INVALID_ARG;
+  if (absent(ctx) || !t3) return ZRL_INVALID_ARG;
   if ((m || v) && count != ctx->flat_params) return bad(ctx, "parameter count mismatch");
   CK(cudaSetDevice(ctx->device));
   std::vector<float> pad(ctx->dev_params);
@@ -1671,7 +1679,7 @@ zrl_status zrl_set_adam_state(zrl_ctx *ctx, const int32_t *t3, const float *m,
 
 zrl_status zrl_get_adam_state(zrl_ctx *ctx, int32_t *t3, float *m, float *v,
                               int64_t count) {
-  if (!ctx || !t3) return ZRL_INVALID_ARG;
+  if (absent(ctx) || !t3) return ZRL_INVALID_ARG;
   if ((m || v) && count != ctx->flat_params) return bad(ctx, "parameter count mismatch");
   CK(cudaSetDevice(ctx->device));
   CK(cudaStreamSynchronize(ctx->stream));
@@ -1694,7 +1702,7 @@ zrl_status zrl_set_normalizers(zrl_ctx *ctx, const float *obs_mean,
                                const float *obs_m2, float obs_count,
                                const float *crit_mean, const float *crit_m2,
                                float crit_count) {
-  if (!ctx || !obs_mean || !obs_m2 || !crit_mean || !crit_m2) return ZRL_INVALID_ARG;
+  if (absent(ctx) || !obs_mean || !obs_m2 || !crit_mean || !crit_m2) return ZRL_INVALID_ARG;
   CK(cudaSetDevice(ctx->device));
   const int od = ctx->net[0].d[0], cd = ctx->net[1].d[0];
   CK(cudaMemcpyAsync(ctx->obs_mean, obs_mean, sizeof(float) * od, cudaMemcpyHostToDevice, ctx->stream));
@@ -1711,7 +1719,7 @@ zrl_status zrl_set_normalizers(zrl_ctx *ctx, const float *obs_mean,
 zrl_status zrl_get_normalizers(zrl_ctx *ctx, float *obs_mean, float *obs_m2,
                                float *obs_count, float *crit_mean, float *crit_m2,
                                float *crit_count) {
-  if (!ctx) return ZRL_INVALID_ARG;
+  if (absent(ctx)) return ZRL_INVALID_ARG;
   CK(cudaSetDevice(ctx->device));
   CK(cudaStreamSynchronize(ctx->stream));
   const int od = ctx->net[0].d[0], cd = ctx->net[1].d[0];
@@ -1725,7 +1733,7 @@ zrl_status zrl_get_normalizers(zrl_ctx *ctx, float *obs_mean, float *obs_m2,
 }
 
 zrl_status zrl_set_lr(zrl_ctx *ctx, float lr) {
-  if (!ctx) return ZRL_INVALID_ARG;
+  if (absent(ctx)) return ZRL_INVALID_ARG;
   CK(cudaSetDevice(ctx->device));
   ctx->lr_host = lr;
   CK(cudaMemcpyAsync(&ctx->st->lr, &ctx->lr_host, sizeof(float), cudaMemcpyHostToDevice,
@@ -1735,7 +1743,7 @@ zrl_status zrl_set_lr(zrl_ctx *ctx, float lr) {
 }
 
 zrl_status zrl_get_lr(zrl_ctx *ctx, float *lr) {
-  if (!ctx || !lr) return ZRL_INVALID_ARG;
+  if (absent(ctx) || !lr) return ZRL_INVALID_ARG;
   CK(cudaSetDevice(ctx->device));
   CK(cudaStreamSynchronize(ctx->stream));
   CK(cudaMemcpy(lr, &ctx->st->lr, sizeof(float), cudaMemcpyDeviceToHost));
@@ -1747,7 +1755,7 @@ zrl_status zrl_gae(zrl_ctx *ctx, const float *rewards, const float *values,
                    const uint8_t *dones, const float *last_values, int64_t n_envs,
                    int64_t T, float gamma, float lam, float *adv_out, float *ret_out,
                    int32_t on_device) {
-  if (!ctx || !rewards || !values || !dones || !last_values || !adv_out || !ret_out)
+  if (absent(ctx) || !rewards || !values || !dones || !last_values || !adv_out || !ret_out)
     return ZRL_INVALID_ARG;
   if (n_envs < 0 || T < 0) return bad(ctx, "negative size");
   if (T > 4096) return bad(ctx, "T larger than 4096 is not supported");
@@ -1840,7 +1848,7 @@ static zrl_status write_back_adv(zrl_ctx *ctx, zrl_batch *b, const float *adv_de
 
 zrl_status zrl_update(zrl_ctx *ctx, const zrl_ppo_config *cfg, zrl_batch *batch,
                       zrl_stats *out) {
-  if (!ctx) return ZRL_INVALID_ARG;
+  if (absent(ctx)) return ZRL_INVALID_ARG;
   TRY(check_cfg(ctx, cfg));
   int64_t n_global = 0;
   TRY(check_batch(ctx, batch, &n_global));
@@ -1861,7 +1869,7 @@ zrl_status zrl_update(zrl_ctx *ctx, const zrl_ppo_config *cfg, zrl_batch *batch,
 
 zrl_status zrl_gae_update(zrl_ctx *ctx, const zrl_ppo_config *cfg,
                           const zrl_rollout *ro, zrl_batch *batch, zrl_stats *out) {
-  if (!ctx || !ro) return ZRL_INVALID_ARG;
+  if (absent(ctx) || !ro) return ZRL_INVALID_ARG;
   TRY(check_cfg(ctx, cfg));
   int64_t n_global = 0;
   TRY(check_batch(ctx, batch, &n_global));
@@ -1915,7 +1923,7 @@ zrl_status zrl_gae_update(zrl_ctx *ctx, const zrl_ppo_config *cfg,
 
 zrl_status zrl_forward(zrl_ctx *ctx, const float *obs, const float *critic_obs,
                        int64_t n, float *mean_out, float *value_out, int32_t on_device) {
-  if (!ctx) return ZRL_INVALID_ARG;
+  if (absent(ctx)) return ZRL_INVALID_ARG;
   if (n < 0) return bad(ctx, "negative n");
   if ((mean_out && !obs) || (value_out && !critic_obs)) return bad(ctx, "null input");
   if (n == 0) return ZRL_OK;
@@ -1965,7 +1973,7 @@ zrl_status zrl_forward(zrl_ctx *ctx, const float *obs, const float *critic_obs,
 }
 
 zrl_status zrl_shuffle_device(zrl_ctx *ctx, uint64_t seed, int64_t n, int32_t *order) {
-  if (!ctx || n < 0 || n > INT32_MAX || (n > 0 && !order)) return ZRL_INVALID_ARG;
+  if (absent(ctx) || n < 0 || n > INT32_MAX || (n > 0 && !order)) return ZRL_INVALID_ARG;
   if (n == 0) return ZRL_OK;
   CK(cudaSetDevice(ctx->device));
   int32_t *scratch = nullptr;
@@ -1985,7 +1993,7 @@ zrl_status zrl_shuffle_device(zrl_ctx *ctx, uint64_t seed, int64_t n, int32_t *o
 int64_t zrl_rank_orders_device(zrl_ctx *ctx, uint64_t seed, int64_t n_global, int64_t n_local,
                                int64_t row_offset, int32_t minibatches, int32_t *order,
                                int64_t *counts) {
-  if (!ctx || n_global <= 0 || n_global > INT32_MAX || minibatches <= 0 || n_local < 0 ||
+  if (absent(ctx) || n_global <= 0 || n_global > INT32_MAX || minibatches <= 0 || n_local < 0 ||
       !order || !counts)
     return -1;
   if (cudaSetDevice(ctx->device) != cudaSuccess) return -1;
@@ -2023,7 +2031,7 @@ int64_t zrl_rank_orders_device(zrl_ctx *ctx, uint64_t seed, int64_t n_global, in
 zrl_status zrl_gemm(zrl_ctx *ctx, int32_t layout, int32_t M, int32_t N, int32_t K,
                     const float *A, int32_t lda, const float *B, int32_t ldb, float *C,
                     int32_t ldc, int32_t split_k) {
-  if (!ctx || !A || !B || !C) return ZRL_INVALID_ARG;
+  if (absent(ctx) || !A || !B || !C) return ZRL_INVALID_ARG;
   if (layout < 0 || layout > 2 || M < 0 || N < 0 || K < 0 || split_k < 1 || split_k > 64)
     return bad(ctx, "invalid GEMM arguments");
   CK(cudaSetDevice(ctx->device));
@@ -2049,7 +2057,7 @@ zrl_status zrl_gemm(zrl_ctx *ctx, int32_t layout, int32_t M, int32_t N, int32_t 
 zrl_status zrl_minibatch_grads(zrl_ctx *ctx, const zrl_ppo_config *cfg,
                                const zrl_batch *batch, const int64_t *idx,
                                int64_t n_idx, float *grads_out, float *sums3_out) {
-  if (!ctx || !idx || !grads_out) return ZRL_INVALID_ARG;
+  if (absent(ctx) || !idx || !grads_out) return ZRL_INVALID_ARG;
   TRY(check_cfg(ctx, cfg));
   int64_t n_global = 0;
   TRY(check_batch(ctx, batch, &n_global));
@@ -2085,7 +2093,7 @@ zrl_status zrl_minibatch_grads(zrl_ctx *ctx, const zrl_ppo_config *cfg,
 
 zrl_status zrl_apply_grads(zrl_ctx *ctx, const zrl_ppo_config *cfg, const float *grads,
                            float kl) {
-  if (!ctx || !grads) return ZRL_INVALID_ARG;
+  if (absent(ctx) || !grads) return ZRL_INVALID_ARG;
   TRY(check_cfg(ctx, cfg));
   CK(cudaSetDevice(ctx->device));
   std::vector<float> pad(ctx->grad_len, 0.0f);
@@ -2103,7 +2111,7 @@ zrl_status zrl_apply_grads(zrl_ctx *ctx, const zrl_ppo_config *cfg, const float 
 zrl_status zrl_set_mirror(zrl_ctx *ctx, const int32_t *obs_perm, const float *obs_sign,
                           const int32_t *cobs_perm, const float *cobs_sign,
                           const int32_t *act_perm, const float *act_sign) {
-  if (!ctx) return ZRL_INVALID_ARG;
+  if (absent(ctx)) return ZRL_INVALID_ARG;
   if (!obs_perm) {
     ctx->mirror = false;
     return ZRL_OK;
@@ -2144,7 +2152,7 @@ zrl_status zrl_set_mirror(zrl_ctx *ctx, const int32_t *obs_perm, const float *ob
 }
 
 zrl_status zrl_set_wait_limit(zrl_ctx *ctx, uint64_t ns) {
-  if (!ctx) return ZRL_INVALID_ARG;
+  if (absent(ctx)) return ZRL_INVALID_ARG;
   if (ns < 1000000ull) return bad(ctx, "wait limit below 1 ms");
   ctx->gemm.wait_ns = ns;
   return ZRL_OK;
@@ -2160,21 +2168,21 @@ zrl_status zrl_test_comm_wait(int32_t scenario, int32_t timeout_ms, int32_t *abo
 }
 
 zrl_status zrl_test_stall_next_gemm(zrl_ctx *ctx) {
-  if (!ctx) return ZRL_INVALID_ARG;
+  if (absent(ctx)) return ZRL_INVALID_ARG;
   if (!ctx->tcore()) return bad(ctx, "the stall hook is in the tensor-core GEMM");
   ctx->gemm.stall_next = 1;
   return ZRL_OK;
 }
 
 zrl_status zrl_set_profiling(zrl_ctx *ctx, int32_t enabled) {
-  if (!ctx) return ZRL_INVALID_ARG;
+  if (absent(ctx)) return ZRL_INVALID_ARG;
   ctx->profiling = enabled != 0;
   return ZRL_OK;
 }
 
 int32_t zrl_profile_site(const zrl_ctx *ctx, int32_t i, const char **name, float *ms,
                          int64_t *spans) {
-  if (!ctx || i < 0 || i >= (int32_t)ctx->sites.size()) return 0;
+  if (absent(ctx) || i < 0 || i >= (int32_t)ctx->sites.size()) return 0;
   if (name) *name = ctx->sites[i].first.c_str();
   if (ms) *ms = ctx->sites[i].second.first;
   if (spans) *spans = ctx->sites[i].second.second;
@@ -2183,7 +2191,7 @@ int32_t zrl_profile_site(const zrl_ctx *ctx, int32_t i, const char **name, float
 
 zrl_status zrl_get_profile(zrl_ctx *ctx, float *gemm_ms, float *update_ms,
                            int64_t *gemm_launches) {
-  if (!ctx) return ZRL_INVALID_ARG;
+  if (absent(ctx)) return ZRL_INVALID_ARG;
   if (gemm_ms) *gemm_ms = ctx->prof_gemm_ms;
   if (update_ms) *update_ms = ctx->prof_update_ms;
   if (gemm_launches) *gemm_launches = ctx->prof_gemm_launches;
@@ -2234,7 +2242,7 @@ static zrl_status fold_rows(zrl_ctx *ctx, const float *x, int64_t n, int dim, fl
 
 static zrl_status record_obs_impl(zrl_ctx *ctx, const float *obs, const float *critic_obs,
                                   int64_t n, int32_t on_device, int32_t mode) {
-  if (!ctx || (n > 0 && (!obs || !critic_obs))) return ZRL_INVALID_ARG;
+  if (absent(ctx) || (n > 0 && (!obs || !critic_obs))) return ZRL_INVALID_ARG;
   if (n < 0) return bad(ctx, "negative n");
   if (mode != 0 && mode != 1) return bad(ctx, "mode must be 0 (sequential) or 1 (parallel)");
   if (n == 0) return ZRL_OK;
@@ -2261,7 +2269,7 @@ zrl_status zrl_record_obs_ex(zrl_ctx *ctx, const float *obs, const float *critic
 
 zrl_status zrl_pending_push(zrl_ctx *ctx, const float *obs, const float *critic_obs, int64_t n,
                             int32_t on_device, int32_t mode) {
-  if (!ctx || (n > 0 && (!obs || !critic_obs))) return ZRL_INVALID_ARG;
+  if (absent(ctx) || (n > 0 && (!obs || !critic_obs))) return ZRL_INVALID_ARG;
   if (n < 0) return bad(ctx, "negative n");
   if (mode != 0 && mode != 1) return bad(ctx, "mode must be 0 (sequential) or 1 (parallel)");
   if (n == 0) return ZRL_OK;
@@ -2277,7 +2285,7 @@ zrl_status zrl_pending_push(zrl_ctx *ctx, const float *obs, const float *critic_
 }
 
 zrl_status zrl_commit_pending(zrl_ctx *ctx) {
-  if (!ctx) return ZRL_INVALID_ARG;
+  if (absent(ctx)) return ZRL_INVALID_ARG;
   CK(cudaSetDevice(ctx->device));
   // a normalizer whose pending state is empty is left as it is (ppo.rs:180)
   if (ctx->pend_obs_count != 0.0f) {
@@ -2302,7 +2310,7 @@ zrl_status zrl_commit_pending(zrl_ctx *ctx) {
 
 zrl_status zrl_get_pending(zrl_ctx *ctx, float *obs_mean, float *obs_m2, float *obs_count,
                            float *crit_mean, float *crit_m2, float *crit_count) {
-  if (!ctx) return ZRL_INVALID_ARG;
+  if (absent(ctx)) return ZRL_INVALID_ARG;
   CK(cudaSetDevice(ctx->device));
   CK(cudaStreamSynchronize(ctx->stream));
   const int od = ctx->net[0].d[0], cd = ctx->net[1].d[0];
@@ -2337,7 +2345,7 @@ static zrl_status policy_step_impl(zrl_ctx *ctx, const float *obs, const float *
                                    int64_t n, uint64_t seed, uint64_t counter, uint64_t *lcg,
                                    float *action, float *logp, float *mean, float *value,
                                    int32_t on_device) {
-  if (!ctx || !obs || !action) return ZRL_INVALID_ARG;
+  if (absent(ctx) || !obs || !action) return ZRL_INVALID_ARG;
   if (value && !critic_obs) return bad(ctx, "value requested without critic_obs");
   if (n < 0) return bad(ctx, "negative n");
   if (n == 0) return ZRL_OK;
@@ -2472,7 +2480,7 @@ static zrl_status build_checkpoint(zrl_ctx *ctx, std::vector<uint8_t> *out) {
 }
 
 zrl_status zrl_save(zrl_ctx *ctx, const char *path) {
-  if (!ctx || !path) return ZRL_INVALID_ARG;
+  if (absent(ctx) || !path) return ZRL_INVALID_ARG;
   std::vector<uint8_t> bytes;
   TRY(build_checkpoint(ctx, &bytes));
   FILE *f = fopen(path, "wb");
@@ -2490,7 +2498,7 @@ zrl_status zrl_save(zrl_ctx *ctx, const char *path) {
 }
 
 zrl_status zrl_load_from_bytes(zrl_ctx *ctx, const uint8_t *bytes, size_t len) {
-  if (!ctx || !bytes) return ZRL_INVALID_ARG;
+  if (absent(ctx) || !bytes) return ZRL_INVALID_ARG;
   std::map<std::string, StTensor> ts;
   if (!st_parse(bytes, len, &ts, &ctx->err)) return ZRL_IO_ERROR;
   std::vector<float> flat(ctx->flat_params);
@@ -2550,7 +2558,7 @@ zrl_status zrl_load_from_bytes(zrl_ctx *ctx, const uint8_t *bytes, size_t len) {
 }
 
 zrl_status zrl_load(zrl_ctx *ctx, const char *path) {
-  if (!ctx || !path) return ZRL_INVALID_ARG;
+  if (absent(ctx) || !path) return ZRL_INVALID_ARG;
   FILE *f = fopen(path, "rb");
   if (!f) {
     ctx->err = std::string("cannot open ") + path;

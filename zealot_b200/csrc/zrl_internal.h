@@ -23,8 +23,10 @@
 namespace zrl {
 
 // Message of this thread's last failed sequence-operator call (they take no
-// context); empty if there is none.
+// context); empty if there is none, or if a call that failed for want of a context
+// came after it.
 const char *seq_last_error();
+void seq_clear_error();
 
 constexpr int kPad = 32;
 inline int64_t pad_to(int64_t x, int64_t a) { return (x + a - 1) / a * a; }
