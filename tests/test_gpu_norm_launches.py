@@ -1,5 +1,5 @@
-"""Group norm as programs launch it: calls of several sizes in one CUDA graph and from
-two host threads."""
+"""Group norm and dropout as programs launch them: calls of several sizes in one
+CUDA graph, on another stream, from two host threads."""
 import threading
 
 import pytest
@@ -81,3 +81,64 @@ def test_block_sizes_from_two_threads(grad):
     for t in threads:
         t.join()
     assert not failed, (len(failed), failed[0])
+
+
+def forms():
+    """Rows; samples in a block; in two passes, one launch and several batches."""
+    g = torch.Generator().manual_seed(3)
+    out = []
+    for shape in ((300, 96), (60, 30, 64), (3, 3000, 64), (9, 60000, 64)):
+        out.append(tuple(torch.randn(shape, generator=g).cuda() for _ in range(2)))
+    return out
+
+
+def drops(x, dy):
+    x, dy = x.view(-1, x.shape[-1]), dy.view(-1, dy.shape[-1])
+    rows = torch.arange(x.shape[0], device="cuda").flip(0)
+    return (S.dropout(x, 0.3, 5, stream=2, rows=rows, residual=dy), S.dropout_grad(dy, 0.3, 5),
+            S.dropout(x[:, :51], 0.5, 6))
+
+
+def test_every_form_in_a_graph():
+    data = forms()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = [both(*d) + drops(*d) for d in data]
+    for d in data:
+        d[0].mul_(0.5), d[1].add_(1.0)
+    for _ in range(2):
+        graph.replay()
+    torch.cuda.synchronize()
+    assert all(same(a, both(*d) + drops(*d)) for a, d in zip(got, data))
+
+
+def test_every_form_on_another_stream():
+    data = forms()
+    want = [both(*d) + drops(*d) for d in data]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = [both(*d) + drops(*d) for d in data]
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    assert all(same(a, b) for a, b in zip(got, want))
+
+
+def test_messages_belong_to_their_thread():
+    x = torch.zeros(4, 16).cuda()
+    seen, met = {}, threading.Barrier(2)
+
+    def work(name, call):
+        with pytest.raises(N.ZrlError):
+            call()
+        met.wait()
+        seen[name] = N.lib().zrl_last_error(None).decode()
+
+    threads = [threading.Thread(target=work, args=a) for a in
+               (("norm", lambda: S.group_norm(x, 4, eps=-1.0)),
+                ("dropout", lambda: S.dropout(x, 2.0, 1)))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert "group_norm" in seen["norm"] and "dropout" in seen["dropout"]

@@ -65,3 +65,39 @@ def test_dlam_of_a_long_row_in_one_piece():
 def test_long_rows_in_one_piece(t, B, T, D):
     kw, dh, dh_last = G.make(B, T, D, t, seed=8, resets=0.005)
     G.check(kw, dh, dh_last, what=f"{B}x{T}x{D} {t}")
+
+
+# A memory of up to some thousand steps.  A step rounds a and h, each by 1.7e-8 at
+# the root mean square, to either side: over the n / 2 steps that an error lives on,
+# 1.6e-7 of h over these decays.  The gates' and rate's roundings, one sided for a
+# channel, come to about 4e-7.  A decay whose rounding has a side would add n / 2
+# times it, several times the bound.
+@pytest.mark.parametrize("B", [1, 300])
+def test_a_long_memory_keeps_its_digits(B):
+    T, D = 20000, 256
+    kw, dh, dh_last = G.make(1, T, D, "f32", seed=2, resets=0, h0=True)
+    x, rec, inp = (kw[k][0].cpu().double() for k in ("x", "rec", "inp"))
+    rate = 8.0 * torch.nn.functional.softplus(kw["lam"].cpu().double(), threshold=1e9)
+    sr, si = torch.sigmoid(rec), torch.sigmoid(inp)
+    a, m = torch.exp(-rate * sr), torch.sqrt(-torch.expm1(-2 * rate * sr))
+    s, h = kw["h0"][0].cpu().double(), torch.empty(T, D, dtype=torch.float64)
+    b = m * si * x
+    for i in range(T):
+        s = a[i] * s + b[i]
+        h[i] = s
+    e, g = dh_last[0].cpu().double(), torch.empty(T, D, dtype=torch.float64)
+    d = dh[0].cpu().double()
+    for i in range(T - 1, -1, -1):
+        e = e + d[i]
+        g[i] = e
+        e = a[i] * e
+    # B rows alike: in slabs, and in one piece
+    wide = {k: v if k == "lam" or v is None else v.expand(B, *v.shape[1:]) for k, v in kw.items()}
+    wide["h0"] = wide["h0"].contiguous()
+    got, last, carry = S.gated_scan(**wide, save=True)
+    dx = S.gated_scan_grad(wide["x"], wide["rec"], wide["inp"], wide["lam"],
+                           dh.expand(B, T, D), carry, dh_last=dh_last.expand(B, D).contiguous(),
+                           h0=wide["h0"])[0]
+    for v, want, bound in ((got, h, 6e-7), (last, s, 6e-7), (dx, g * m * si, 8e-7)):
+        off = (v[-1].cpu().double() - want).norm() / want.norm()
+        assert off <= bound, (v.shape, off.item())
