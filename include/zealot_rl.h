@@ -446,7 +446,8 @@ typedef enum {
  * rstd = 1 / sqrt(population variance + eps); C at most 2^23.  gamma, beta [C] fp32 or NULL
  * (1, 0).  mean, rstd [N, groups] or NULL: what the gradient needs.  strides:
  * (n, l) of x and y, four in all.  y may be x (same strides).  workspace:
- * zrl_group_norm_workspace(..., 0) bytes, 16-byte aligned (NULL if 0).  No
+ * zrl_group_norm_workspace(..., 0) bytes, 16-byte aligned (NULL if 0).  ELU and
+ * GELU keep the digits of a small result, up to the rounding of z.  No
  * counterpart in the reference. */
 zrl_status zrl_group_norm(const void *x, const float *gamma, const float *beta,
                           int64_t N, int64_t L, int64_t C, int32_t groups,
@@ -465,7 +466,10 @@ zrl_status zrl_group_norm_grad(const void *x, const void *dy, const float *gamma
                                float *dbeta, void *workspace,
                                int64_t workspace_bytes, void *stream);
 /* Bytes of the workspace of zrl_group_norm (grad 0) or zrl_group_norm_grad
- * (grad 1).  No counterpart in the reference. */
+ * (grad 1).  The gradient's grows with N where a sample has several rows, or one
+ * with groups of more than 256 fp32 or 512 16-bit channels (128 at odd widths):
+ * 8 C bytes a sample at least, more than x itself takes there.  No counterpart in the
+ * reference. */
 int64_t zrl_group_norm_workspace(int64_t N, int64_t L, int64_t C, int32_t groups,
                                  int32_t grad);
 

@@ -30,8 +30,10 @@ constexpr float kSeriesMax = 0.35f;
 constexpr float kSmallest = 1.17549435e-38f;  // 2^-126
 
 // Blocks of 256 threads an SM holds, which bounds their registers.  Measured
-// (device us, 2 / 3 / 4 blocks): forward 1024 x 24 x 512 bf16 35 / 34 / 32, 4096 x
-// 24 x 128 f32 41 / 47 / 55 (spills); gradient of the former 49 / 110 / - (spills).
+// (device us, 2 / 3 / 4 blocks): forward 1024 x 24 x 512 bf16 36 / 34 / 32, 4096 x
+// 24 x 128 f32 42 / 48 / 55; gradient of the former 50 / 118 / -.  The fastest of
+// them spill as well, less than they gain: bf16 pairs store / load 124 / 208 bytes a
+// thread in scan_kernel, 140 / 144 in the first pass, 56 / 84 in the gradient.
 template <typename T> constexpr int resident() { return sizeof(T) == 2 ? 4 : 2; }
 // (f32's gradient takes one channel a lane: pairs spill, 78 against 106 us.)
 constexpr int kGradResident = 2;
@@ -75,7 +77,7 @@ __device__ __forceinline__ float softplus(float v) {
 enum Way { kPlain, kMarks, kFar };
 template <Way W> using Is = std::integral_constant<Way, W>;
 // Whether scan_kernel has a path of its own for kMarks.  Device us with / without:
-// 1024 x 24 x 512 bf16 32 / 35 (fewer spills), 4096 x 24 x 128 f32 43 / 41.  The fold
+// 1024 x 24 x 512 bf16 32 / 35 (fewer spills), 4096 x 24 x 128 f32 44 / 42.  The fold
 // and the gradient are faster without: 8 x 8191 x 480 bf16 62 / 61 and 128 / 125.
 template <typename T> constexpr bool kMarksApart = sizeof(T) == 2;
 
@@ -267,10 +269,10 @@ struct Slab {
 // What a slab does to the state before it (BACK: to the gradient after it), as a
 // pair (P, H): every warp folds its slab, then the block writes, per warp, the
 // pair of the block's slabs before (after) it, and the pair of them all.
-// Bound by the special functions and the issue slots (about 33 a step and
-// channel) where elements have two bytes, by memory where they have four:
-// 1 x 65536 x 512 f32 71 us (5.7 TB/s), 8 x 8191 x 480 bf16 60 us (3.1 TB/s; the
-// special functions at 57 % of their rate), backwards 43 us.
+// Bound by memory where elements have four bytes: 1 x 65536 x 512 f32 72 us (5.6
+// TB/s).  Where they have two no unit is full: 8 x 8191 x 480 bf16 65 us (2.9 TB/s),
+// backwards 43 us, the special functions at 66 and 43 % of their rate, 55 and 59 %
+// of the issue slots, and warps that mostly wait for their loads.
 template <typename T, int V, bool BACK>
 __global__ void __launch_bounds__(256, resident<T>()) scan_fold_kernel(const __grid_constant__ ScanArgs a) {
   constexpr int S = kSteps;
@@ -395,10 +397,12 @@ __device__ __forceinline__ void enter_slab(const ScanArgs &a, const Slab &slab, 
 // A thread takes its V channels through the steps of its slab, with the loads
 // of the eight steps ahead in flight: each step's gates are independent work, only
 // one multiply-add a step is in sequence, and nothing is exchanged.  Measured:
-// 4096 x 24 x 128 f32 41 us (4.9 TB/s), 1024 x 24 x 512 bf16 32 us (3.3 TB/s: about 38
-// issue slots and four special functions a step and channel at 42 % of the warps
-// its registers allow), 1 x 65536 x 512 f32 85 us (6.3 TB/s).  Blocks that split the
-// steps of a tile among warps and met in shared memory took 59, 55 and 278 us.
+// 4096 x 24 x 128 f32 42 us (4.8 TB/s), 1024 x 24 x 512 bf16 32 us (3.3 TB/s), 1 x
+// 65536 x 512 f32 86 us (6.3 TB/s).  The last is bound by memory; the others wait for
+// loads, with what 16 (f32) and 32 warps an SM can keep in flight: in bf16 57 % of the
+// issue slots and of the special functions' rate, five of them a step and channel.
+// Blocks that split the steps of a tile among warps and met in shared memory took 59,
+// 55 and 278 us.
 template <typename T, int V>
 __global__ void __launch_bounds__(256, resident<T>()) scan_kernel(const __grid_constant__ ScanArgs a) {
   constexpr int S = kSteps;
@@ -485,9 +489,10 @@ __global__ void __launch_bounds__(256, resident<T>()) scan_kernel(const __grid_c
 // stretch, g_t = dh_t + gamma_{t+1}, gamma_t = a_t g_t, from the decays alone;
 // then forwards, with the states running on from the kept one and every output
 // made as its step comes by.  So every gate is computed once and only the decay,
-// sigmoid(rec) and g of a stretch are held.  Bound by issue slots (72 a step and
-// channel) at the sixteen warps an SM that its registers allow: 1024 x 24 x 512 bf16
-// 49 us (3.7 TB/s), 8 x 8191 x 480 bf16 125 us (3.6 TB/s).
+// sigmoid(rec) and g of a stretch are held.  1024 x 24 x 512 bf16 50 us (3.6 TB/s), 8 x
+// 8191 x 480 bf16 126 us (3.6 TB/s), at 56 and 52 % of the issue slots: with the sixteen
+// warps an SM that its registers allow, of which 3.5 a scheduler run, it waits for
+// loads and for its own chains of products in about equal parts.
 template <typename T, int V>
 __global__ void __launch_bounds__(256, kGradResident)
     scan_grad_kernel(const __grid_constant__ ScanArgs a) {

@@ -62,6 +62,12 @@ struct NormShape {
 //           (98304 x 250 forward, vector by vector; 53 us now).
 //  block:   a sample's columns fit a block's shared memory.
 //  passes:  the rest.
+// A row whose groups are too wide for the lanes of a warp (above 256 channels in fp32
+// and 512 in 16 bits on aligned rows, 128 at odd widths) goes to the block form with one
+// position, which is made for many: 24576 x 1024 bf16 in one group 316 us forward and
+// 378 us with its sums back, where 512 channels take 16 and 49; so are samples of a few
+// positions (16384 x 4 x 256 bf16 259 and 309 us).  And the block form leaves its sums per
+// sample: a gradient's workspace of 2 C floats for each of N.
 struct NormPlan {
   enum { kLanes, kBlock, kPasses } form;
   int vec, E, p, gb, rb, blocks, across;  // lanes

@@ -8,8 +8,10 @@
 namespace zrl {
 namespace {
 
-// Resident blocks, which bounds the registers.  Three spill where a lane has four
-// single channels: 98304 x 250 f32 forward 62 -> 109 us.
+// Resident blocks, which bounds the registers; one number for all forms.  Three spill
+// where a lane has four single channels: 98304 x 250 f32 forward 62 -> 109 us.  (Not
+// measured for the forms of one vector a lane, which have room.  At two, the gradient
+// with two vectors of eight channels spills: 276 bytes a thread stored, 148 loaded.)
 constexpr int kLaneBlocks = 2;
 
 template <int VEC, int V>
@@ -62,10 +64,11 @@ struct RowLanes {
 
 // U rows rb apart at a time; the next ones' loads are in flight.  A lane's vectors
 // are taken as one, so that single channels go through the packed instructions
-// too.  Bound by issue slots at the sixteen warps an SM that its registers allow:
-// 24576 x 512 bf16 in groups of 32 ELU 12 us (4.2 TB/s), 98304 x 250 f32 in groups of
-// 25 SiLU 53 us (3.7 TB/s; vector by vector 62, rows staged as flat tiles in shared
-// memory 70).
+// too.  24576 x 512 bf16 in groups of 32 ELU 14 us (3.7 TB/s), 98304 x 250 f32 in groups
+// of 25 SiLU 53 us (3.7 TB/s; vector by vector 62, rows staged as flat tiles in shared
+// memory 70), at 63 and 66 % of the issue slots: sixteen warps an SM, the most that its
+// registers allow, do not cover the latency of one product after the other and of
+// the sums' shuffles.
 template <typename T, int VEC, int E>
 __global__ void __launch_bounds__(kThreads, kLaneBlocks)
     norm_rows_kernel(const __grid_constant__ NormArgs a) {
@@ -135,8 +138,9 @@ __global__ void __launch_bounds__(kThreads, kLaneBlocks)
 }
 
 // dx, and part[block][2][C]: the block's sums for dgamma and dbeta, kept in
-// registers over all its rows.  98304 x 250 f32 in groups of 25 SiLU 101 us (2.9
-// TB/s; 119 with a lane's vectors taken as one: its loads are waited for longer).
+// registers over all its rows.  98304 x 250 f32 in groups of 25 SiLU 102 us (2.9
+// TB/s; 119 with a lane's vectors taken as one), 58 % of the issue slots: single
+// elements a load, which are waited for.
 template <typename T, int VEC, int E>
 __global__ void __launch_bounds__(kThreads, kLaneBlocks)
     norm_rows_grad_kernel(const __grid_constant__ NormArgs a) {

@@ -285,7 +285,9 @@ struct Scale {
 };
 
 // Second pass: the pieces' means and squares give the group's, then y.  64 x 5046 x
-// 64 f16 ELU 16 us, 16 x 6360 x 256 bf16 GELU 27 us (23 issue slots a value).
+// 64 f16 ELU 19 us, 16 x 6360 x 256 bf16 GELU 28 us, at 67 and 62 % of the issue
+// slots: its warps mostly wait for their turn at them, and the rest is the start and
+// the end of the blocks.
 template <typename T, int VEC>
 __global__ void __launch_bounds__(kThreads, sample_blocks(false))
     norm_apply_kernel(const __grid_constant__ NormArgs a) {
@@ -404,8 +406,9 @@ __device__ __forceinline__ void grad_sums(const NormArgs &a, const Patch<VEC> &k
 }
 
 // Gradient, first pass: grad_sums, the groups' into means[n][group][piece].  16 x
-// 6360 x 256 bf16 GELU 33 us (3.1 TB/s; 31 without the block's sums, and no more
-// without the GELU); four positions a turn take as long.
+// 6360 x 256 bf16 GELU 35 us (3.0 TB/s), 56 % of the issue slots at 29 % of the warps
+// (31 without the block's sums, and no more without the GELU, where it took 33); four
+// positions a turn take as long.
 template <typename T, int VEC>
 __global__ void __launch_bounds__(kThreads, sample_blocks(true))
     norm_grad_sums_kernel(const __grid_constant__ NormArgs a) {
@@ -446,7 +449,7 @@ __device__ __forceinline__ void write_dx(const Slope<VEC> &slope, const Vec<VEC>
   dx.next();
 }
 
-// Gradient, second pass: dx.  As the first 38 us.
+// Gradient, second pass: dx.  As the first 41 us, 58 % of the issue slots.
 template <typename T, int VEC>
 __global__ void __launch_bounds__(kThreads, sample_blocks(true))
     norm_grad_apply_kernel(const __grid_constant__ NormArgs a) {
@@ -493,7 +496,7 @@ __global__ void __launch_bounds__(kThreads, sample_blocks(true))
 // ------------------------------------------------ samples held by a block
 
 // The block keeps what it read in shared memory; a thread reads back only its
-// own.  200 x 300 x 96 bf16 11 us (2.1 TB/s), latency of one turn of the blocks.
+// own.  200 x 300 x 96 bf16 ELU 12.5 us (1.8 TB/s), latency of one turn of the blocks.
 // Clusters of up to 16 blocks that held larger samples together and exchanged sums
 // took 34 us for 64 x 5046 x 64 f16, where two passes take 28.
 template <typename T, int VEC>
