@@ -468,8 +468,8 @@ zrl_status zrl_group_norm_grad(const void *x, const void *dy, const float *gamma
 /* Bytes of the workspace of zrl_group_norm (grad 0) or zrl_group_norm_grad
  * (grad 1).  The gradient's grows with N where a sample has several rows, or one
  * with groups of more than 256 fp32 or 512 16-bit channels (128 at odd widths):
- * 8 C bytes a sample at least, more than x itself takes there.  No counterpart in the
- * reference. */
+ * 8 C bytes a sample at least, which for a few rows is as much as x or more.  No
+ * counterpart in the reference. */
 int64_t zrl_group_norm_workspace(int64_t N, int64_t L, int64_t C, int32_t groups,
                                  int32_t grad);
 
